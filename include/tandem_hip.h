@@ -365,6 +365,26 @@ int tdm_k4_unit_gather(void* full, const void* const* shards, const int64_t* siz
 int tdm_k4_unit_gather_all(void* const* fulls, const void* const* shards, const int64_t* sizes, int world, int dtype,
                            tdm_stream stream);
 
+/* ---- K5: the embedding lookup with a scale, and its gradient -------------- */
+
+/* The model operators (tdm_k5_*, tdm_k6_*, tdm_k7_*) have no counterpart among the reference's kernels: its model
+ * (tandem/model.py:14-120) is made of torch's own. They take TDM_F32, TDM_F16 and TDM_BF16, sum in fp32 and round once. Every
+ * pointer needs its element's alignment only, unless it says otherwise; what a launcher needs beyond its operands is a
+ * workspace of the caller's, which it may fill with anything, and which two launches that can run at the same time must not share.
+ *
+ * out[i, :] = scale * weight[tokens[i], :] for i < n; weight [vocab, dim], out [n, dim], both contiguous. Tokens are
+ * TDM_I64 or TDM_I32 (index_dtype). A token outside [0, vocab) reads nothing; its row of out is NaN. */
+int tdm_k5_embedding(const void* weight, const void* tokens, int index_dtype, void* out, int64_t n, int64_t vocab, int64_t dim, int dtype,
+                     float scale, tdm_stream stream);
+
+/* dweight[v, :] = scale * the sum of grad[i, :] over the i with tokens[i] = v, in the order of i, summed in fp32 and rounded
+ * once: the same bits every time. All of dweight [vocab, dim] is written; a row without a token is zero. The token
+ * `padding` (-1: none) and tokens outside [0, vocab) take no gradient. The workspace starts on 16 bytes and holds
+ * tdm_k5_embedding_grad_workspace(n, vocab, dim) bytes (-1: arguments out of range). */
+int64_t tdm_k5_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t dim);
+int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype, void* dweight, void* workspace, int64_t workspace_bytes,
+                          int64_t n, int64_t vocab, int64_t dim, int dtype, float scale, int64_t padding, tdm_stream stream);
+
 /* ---- the engine: Group(backend="hip") --------------------------------------- */
 
 /* One rank's half of a group whose ranks are processes sharing one GPU. Mirrors
