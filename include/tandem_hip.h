@@ -385,6 +385,51 @@ int64_t tdm_k5_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t dim);
 int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype, void* dweight, void* workspace, int64_t workspace_bytes,
                           int64_t n, int64_t vocab, int64_t dim, int dtype, float scale, int64_t padding, tdm_stream stream);
 
+/* ---- K6: norms of queries and keys per head, with the position rotation ---- */
+
+/* Heads of head_dim contiguous elements: element d of head h of token t of sequence b lies at
+ * data + b * batch_stride + t * token_stride + h * head_stride + d (strides in elements; 0 repeats). */
+typedef struct tdm_heads {
+  void* data;
+  int64_t batch_stride, token_stride, head_stride;
+} tdm_heads;
+
+/* The position of token t of sequence b: data[b * batch_stride + t * token_stride], TDM_I64 or TDM_I32. */
+typedef struct tdm_positions {
+  const void* data;
+  int64_t batch_stride, token_stride;
+} tdm_positions;
+
+typedef struct tdm_qk_shape {
+  int64_t batch, tokens;           /* sequences, tokens of each; fewer than 2^31 tokens in all */
+  int32_t q_heads, kv_heads;       /* of every token; 0: none */
+  int32_t head_dim, rotary_dim;    /* even; head_dim at most 512; the first rotary_dim elements of a head are rotated */
+  int32_t interleaved;             /* pairs are elements 2i and 2i + 1; otherwise i and i + rotary_dim / 2 */
+  int32_t dtype, weight_dtype;     /* of the heads; of the weights: the same or TDM_F32 */
+  int32_t position_dtype;
+  float eps;
+} tdm_qk_shape;
+
+/* Every query and key head x becomes y = x / sqrt(mean(x^2) + eps) * weight (weight [head_dim]; NULL: ones), then every pair
+ * (a, b) of its rotated elements (a cos - b sin, b cos + a sin) of the angle position * inv_freq[i], i the pair's number (inv_freq:
+ * rotary_dim / 2 doubles in GPU memory; the angle is computed in doubles). One pass: x read once, y written once. q_out may be q
+ * and k_out may be k. */
+int tdm_k6_qk_norm_rope(const tdm_qk_shape* shape, const tdm_heads* q, const tdm_heads* k, const void* q_weight, const void* k_weight,
+                        const tdm_positions* positions, const double* inv_freq, const tdm_heads* q_out, const tdm_heads* k_out,
+                        tdm_stream stream);
+
+/* Its gradient: dq, dk for the upstream gradients dq_out, dk_out (data NULL: zeros), from the q and k that went in, and
+ * dq_weight, dk_weight [head_dim] in weight_dtype (NULL: not wanted), summed in fp32 over all tokens and heads in a fixed
+ * order. Where dv has data, dv_out (data NULL: zeros; NULL itself too) is copied there, head for head, in the same pass: the
+ * gradient of a packed q | k | v is then written whole. The workspace starts on 16 bytes and holds
+ * tdm_k6_qk_norm_rope_grad_workspace(shape) bytes (-1: arguments out of range). */
+int64_t tdm_k6_qk_norm_rope_grad_workspace(const tdm_qk_shape* shape);
+int tdm_k6_qk_norm_rope_grad(const tdm_qk_shape* shape, const tdm_heads* dq_out, const tdm_heads* dk_out, const tdm_heads* dv_out,
+                             const tdm_heads* q, const tdm_heads* k, const void* q_weight, const void* k_weight,
+                             const tdm_positions* positions, const double* inv_freq, const tdm_heads* dq, const tdm_heads* dk,
+                             const tdm_heads* dv, void* dq_weight, void* dk_weight, void* workspace, int64_t workspace_bytes,
+                             tdm_stream stream);
+
 /* ---- the engine: Group(backend="hip") --------------------------------------- */
 
 /* One rank's half of a group whose ranks are processes sharing one GPU. Mirrors

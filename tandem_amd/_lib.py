@@ -56,6 +56,22 @@ class AdamwHyper(ctypes.Structure):
                 ("eps", ctypes.c_double), ("neg_step", ctypes.c_double)]
 
 
+class HeadsView(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Positions(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64)]
+
+
+class QkShape(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("weight_dtype", ctypes.c_int32), ("position_dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+_PHEADS, _PSHAPE, _PPOSITIONS = ctypes.POINTER(HeadsView), ctypes.POINTER(QkShape), ctypes.POINTER(Positions)
+
 _SIGNATURES = {
     "tdm_last_error": (ctypes.c_char_p, []),
     "tdm_abi_version": (ctypes.c_int, []),
@@ -116,6 +132,12 @@ _SIGNATURES = {
     "tdm_k5_embedding_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_int64,
                                              ctypes.c_void_p]),
+    "tdm_k6_qk_norm_rope": (ctypes.c_int, [_PSHAPE, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p, _PPOSITIONS, ctypes.c_void_p,
+                                           _PHEADS, _PHEADS, ctypes.c_void_p]),
+    "tdm_k6_qk_norm_rope_grad_workspace": (ctypes.c_int64, [_PSHAPE]),
+    "tdm_k6_qk_norm_rope_grad": (ctypes.c_int, [_PSHAPE, _PHEADS, _PHEADS, _PHEADS, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p,
+                                                _PPOSITIONS, ctypes.c_void_p, _PHEADS, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
 }
 
 _lib = None

@@ -1,5 +1,5 @@
 """The operators of the model that torch has no single pass for, as HIP kernels: the embedding lookup with a scale and its
-gradient by sorted tokens.
+gradient by sorted tokens; the norms of queries and keys per head with the position rotation in the same pass.
 
 Functions on tensors in GPU memory, differentiable, launched on the current stream of the tensors' device; float32,
 float16 and bfloat16, sums in fp32, one rounding at the end. Each has its gradient beside it (`*_grad`) for programs that
@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from ._lib import check, dtype_code, lib, require_device_tensor, stream_ptr
+from ._lib import HeadsView, Positions, QkShape, check, dtype_code, lib, require_device_tensor, stream_ptr
 
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 INDEX_DTYPES = (torch.int64, torch.int32)
@@ -130,3 +130,195 @@ class _Embedding(torch.autograd.Function):
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
         return None, _embedding_grad(grad.contiguous(), tokens, *ctx.how), None, None
+
+
+# ---- norms of queries and keys, with the rotation
+
+
+def rope_frequencies(rotary_dim, base=10000.0, device="cuda"):
+    """The rotation's angles per position: base ** (-2 i / rotary_dim) for i < rotary_dim / 2, float64."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"an even number of rotated elements, not {rotary_dim}")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    return (base ** (-i / rotary_dim)).to(device)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """Every head of q [batch, tokens, q_heads, dim] and k [batch, tokens, kv_heads, dim] (or both without batch) divided by the
+    root of its mean square (+ eps), times its weight [dim] (None: ones), and rotated by its token's position: the pairs
+    (a, b) of its first 2 * len(inv_freq) elements become (a cos - b sin, b cos + a sin) of position * inv_freq[i]. A pair is
+    elements i and i + len(inv_freq); with `interleaved` 2i and 2i + 1. Returns (q, k) of the same shapes, contiguous.
+
+    q and k may be views of any strides whose last dimension is contiguous; float32, float16 or bfloat16, the weights of the
+    same dtype or float32. positions: int64 or int32, of a shape that expands to [batch, tokens]; inv_freq: float64
+    (rope_frequencies). Angles are computed in float64, so far positions keep their precision. Single tokens are a
+    batch of one token each."""
+    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, how)
+    return _qk_forward(q, k, q_weight, k_weight, how)
+
+
+def qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """The gradients (dq, dk, dq_weight, dk_weight) of qk_norm_rope for the upstream gradients dq_out, dk_out (None: zeros); a
+    weight that is None has none. The weights' gradients are summed in fp32 over all tokens and heads in a fixed order."""
+    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    dq, dk = torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, k, q_weight, k_weight, how, dq, dk, None))
+
+
+def qkv_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """qk_norm_rope on a packed projection: qkv [batch, tokens, (q_heads + 2 kv_heads) * dim] (or without batch) holds the
+    queries' heads, the keys' and the values'. Returns (q, k, v): q and k as qk_norm_rope does, v a view of qkv. Its gradient
+    is one pass that writes the gradient of qkv whole, the values' part included."""
+    q, k, v = _split_qkv(qkv, q_heads, kv_heads)
+    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight)):
+        return _QkvNormRope.apply(qkv, q_heads, kv_heads, q_weight, k_weight, how)
+    return (*_qk_forward(q, k, q_weight, k_weight, how), v)
+
+
+def qkv_norm_rope_grad(dq_out, dk_out, dv_out, qkv, q_heads, kv_heads, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
+    """The gradients (dqkv, dq_weight, dk_weight) of qkv_norm_rope for the upstream gradients dq_out, dk_out, dv_out (None: zeros)."""
+    q, k, v = _split_qkv(qkv, q_heads, kv_heads)
+    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
+    return (dqkv, *_qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, how, *_split_qkv(dqkv, q_heads, kv_heads)))
+
+
+def _split_qkv(qkv, q_heads, kv_heads):
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() not in (2, 3):
+        raise ValueError("qkv: [batch, tokens, width] or [tokens, width]")
+    heads = q_heads + 2 * kv_heads
+    if q_heads < 1 or kv_heads < 1 or qkv.shape[-1] == 0 or qkv.shape[-1] % heads:
+        raise ValueError(f"qkv: a width of {qkv.shape[-1]} for {q_heads} query heads and {kv_heads} key and value heads")
+    if qkv.stride(-1) != 1:
+        raise ValueError("qkv: the last dimension must be contiguous")
+    x = qkv.unflatten(-1, (heads, -1))
+    return x[..., :q_heads, :], x[..., q_heads:q_heads + kv_heads, :], x[..., q_heads + kv_heads:, :]
+
+
+class _QkHow:
+    """What a call and its gradient share besides the tensors they differentiate."""
+
+    __slots__ = ("shape", "positions", "at", "inv_freq")
+
+
+def _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved):
+    for t, what in ((q, "q"), (k, "k")):
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+            raise ValueError(f"qk_norm_rope({what}): needs a tensor in GPU memory (got {getattr(t, 'device', type(t))}); tandem_amd has no CPU path")
+        if t.dtype not in DTYPES:
+            raise ValueError(f"qk_norm_rope({what}): float32, float16 or bfloat16, not {t.dtype}")
+        if t.dim() not in (3, 4) or 0 in t.shape[-2:] or t.stride(-1) != 1:
+            raise ValueError(f"qk_norm_rope({what}): [batch, tokens, heads, dim] or [tokens, heads, dim], the last dimension contiguous")
+    if q.dtype != k.dtype or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"q {list(q.shape)} {q.dtype} and k {list(k.shape)} {k.dtype} differ in dtype, tokens or head size")
+    dim = q.shape[-1]
+    weight_dtype = q.dtype
+    for w in (q_weight, k_weight):
+        if w is None:
+            continue
+        _floating(w, "qk_norm_rope(weight)")
+        if w.shape != (dim,) or w.dtype not in (q.dtype, torch.float32):
+            raise ValueError(f"a weight of {list(w.shape)} {w.dtype} for heads of {dim} {q.dtype}")
+        weight_dtype = w.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("q_weight and k_weight differ in dtype")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in INDEX_DTYPES:
+        raise ValueError("positions: an int64 or int32 tensor")
+    require_device_tensor(inv_freq, "qk_norm_rope(inv_freq)")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > dim:
+        raise ValueError(f"inv_freq: at most {dim // 2} float64 values")
+    _same_device(q, k, q_weight, k_weight, positions, inv_freq)
+    tokens = q.shape[:-2]
+    how = _QkHow()
+    if positions.shape != tokens:
+        try:
+            positions = positions.expand(tokens)
+        except RuntimeError:
+            raise ValueError(f"positions of {list(positions.shape)} for tokens of {list(tokens)}") from None
+    how.positions, how.inv_freq = positions, inv_freq
+    strides = positions.stride() if len(tokens) == 2 else (0, *positions.stride())
+    how.at = Positions(positions.data_ptr(), *strides)
+    batch = tokens[0] if len(tokens) == 2 else 1
+    how.shape = QkShape(batch, tokens[-1], q.shape[-2], k.shape[-2], dim, 2 * inv_freq.numel(), int(interleaved), dtype_code(q.dtype),
+                        dtype_code(weight_dtype), dtype_code(positions.dtype), eps)
+    return how
+
+
+def _heads(t):
+    if t is None:
+        return HeadsView()
+    return HeadsView(t.data_ptr(), *(t.stride()[:-1] if t.dim() == 4 else (0, *t.stride()[:-1])))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _qk_forward(q, k, q_weight, k_weight, how):
+    q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    k_out = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    _call(q.device, lib().tdm_k6_qk_norm_rope, how.shape, _heads(q), _heads(k), _ptr(q_weight), _ptr(k_weight), how.at,
+          how.inv_freq.data_ptr(), _heads(q_out), _heads(k_out))
+    return q_out, k_out
+
+
+def _upstream(g, like, what):
+    """An upstream gradient as the kernel reads it: of any strides, the last dimension contiguous."""
+    if g is None:
+        return None
+    if g.shape != like.shape or g.dtype != like.dtype or g.device != like.device:
+        raise ValueError(f"{what}: a gradient of {list(g.shape)} {g.dtype} on {g.device} for {list(like.shape)} {like.dtype} on {like.device}")
+    return g if g.stride(-1) == 1 else g.contiguous()
+
+
+def _qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, how, dq, dk, dv):
+    dq_out, dk_out = _upstream(dq_out, q, "dq_out"), _upstream(dk_out, k, "dk_out")
+    dv_out = None if dv is None else _upstream(dv_out, dv, "dv_out")
+    L = lib()
+    need = L.tdm_k6_qk_norm_rope_grad_workspace(how.shape)
+    if need < 0:
+        raise ValueError(L.tdm_last_error().decode(errors="replace"))
+    work = torch.empty(need, device=q.device, dtype=torch.uint8)
+    dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+    _call(q.device, L.tdm_k6_qk_norm_rope_grad, how.shape, _heads(dq_out), _heads(dk_out), _heads(dv_out), _heads(q), _heads(k),
+          _ptr(q_weight), _ptr(k_weight), how.at, how.inv_freq.data_ptr(), _heads(dq), _heads(dk), _heads(dv), _ptr(dqw), _ptr(dkw),
+          work.data_ptr(), need)
+    return dqw, dkw
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, how):
+        ctx.save_for_backward(q, k, q_weight, k_weight, how.positions, how.inv_freq)
+        ctx.how = how
+        ctx.set_materialize_grads(False)
+        return _qk_forward(q, k, q_weight, k_weight, how)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight = ctx.saved_tensors[:4]
+        dq, dk = torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, k, q_weight, k_weight, ctx.how, dq, dk, None), None)
+
+
+class _QkvNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, q_heads, kv_heads, q_weight, k_weight, how):
+        ctx.save_for_backward(qkv, q_weight, k_weight, how.positions, how.inv_freq)
+        ctx.heads, ctx.how = (q_heads, kv_heads), how
+        ctx.set_materialize_grads(False)
+        q, k, v = _split_qkv(qkv, q_heads, kv_heads)
+        return (*_qk_forward(q, k, q_weight, k_weight, how), v)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out, dv_out):
+        qkv, q_weight, k_weight = ctx.saved_tensors[:3]
+        q, k, _ = _split_qkv(qkv, *ctx.heads)
+        dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
+        grads = _qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, ctx.how, *_split_qkv(dqkv, *ctx.heads))
+        return (dqkv, None, None, *grads, None)

@@ -45,3 +45,47 @@ def test_embedding_argument_errors_need_no_gpu():
     refused(grad(p, p, i64, p, ctypes.c_void_p(4100), need, 10_000, 4, 4, f32, 1.0, -1), "16 bytes")
     refused(grad(p, p, i64, None, p, need, 10_000, 4, 4, f32, 1.0, -1), "null")
     refused(grad(p, p, 7, p, p, need, 10_000, 4, 4, f32, 1.0, -1), "int64")
+
+
+def test_qk_norm_rope_refuses_cpu_tensors_and_odd_rotations():
+    from tandem_amd import ops
+
+    q, freq = torch.zeros(1, 2, 3, 64), torch.zeros(32, dtype=torch.float64)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.qk_norm_rope(q, q, None, None, torch.arange(2), freq)
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.qkv_norm_rope(torch.zeros(1, 2, 192), 1, 1, None, None, torch.arange(2), freq)
+    with pytest.raises(ValueError, match="even"):
+        ops.rope_frequencies(63, device="cpu")
+    f = ops.rope_frequencies(8, base=100.0, device="cpu")
+    assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 10 ** -0.5, 0.1, 10 ** -1.5], dtype=torch.float64), rtol=1e-14)
+
+
+def test_qk_norm_rope_argument_errors_need_no_gpu():
+    lib = _lib()
+    L = lib.lib()
+    assert ctypes.sizeof(lib.HeadsView) == 32 and ctypes.sizeof(lib.Positions) == 24 and ctypes.sizeof(lib.QkShape) == 56
+
+    def shape(**change):
+        s = lib.QkShape(1, 2, 4, 2, 64, 64, 0, 3, 3, 4, 1e-6)
+        for name, value in change.items():
+            setattr(s, name, value)
+        return s
+
+    h, at, p = lib.HeadsView(4096, 128, 64, 64), lib.Positions(4096, 0, 1), ctypes.c_void_p(4096)  # never read
+    call = lambda s, **k: L.tdm_k6_qk_norm_rope(s, k.get("q", h), h, p, p, k.get("at", at), k.get("freq", p), h, h, None)  # noqa: E731
+    for change, word in ((dict(dtype=1), "dtype"), (dict(weight_dtype=2), "weights"), (dict(position_dtype=0), "positions"), (dict(tokens=1 << 31), "tokens"),
+                         (dict(batch=-1), "tokens"), (dict(q_heads=-1), "heads"), (dict(head_dim=63), "even"), (dict(head_dim=514), "512"),
+                         (dict(rotary_dim=66), "rotated"), (dict(rotary_dim=3), "rotated"), (dict(eps=-1.0), "eps")):
+        refused(call(shape(**change)), word)
+        assert L.tdm_k6_qk_norm_rope_grad_workspace(shape(**change)) == -1
+    refused(call(shape(), q=lib.HeadsView()), "null")
+    refused(call(shape(), at=lib.Positions()), "null")
+    refused(call(shape(), freq=None), "null")
+    assert call(shape(tokens=0), q=lib.HeadsView()) == 0
+    need = L.tdm_k6_qk_norm_rope_grad_workspace(shape())
+    assert need >= 2 * 64 * 4
+    grad = lambda w, n: L.tdm_k6_qk_norm_rope_grad(shape(), h, h, None, h, h, p, p, at, p, h, h, None, p, p, w, n, None)  # noqa: E731
+    refused(grad(p, need - 1), "workspace")
+    refused(grad(None, need), "workspace")
+    refused(grad(ctypes.c_void_p(4100), need), "workspace")
