@@ -430,6 +430,40 @@ int tdm_k6_qk_norm_rope_grad(const tdm_qk_shape* shape, const tdm_heads* dq_out,
                              const tdm_heads* dv, void* dq_weight, void* dk_weight, void* workspace, int64_t workspace_bytes,
                              tdm_stream stream);
 
+/* ---- K7: the distillation loss from a teacher's top logits, with its gradient ---- */
+
+enum tdm_distill_reduction { TDM_DISTILL_NONE = 0, TDM_DISTILL_MEAN = 1, TDM_DISTILL_SUM = 2 };
+
+typedef struct tdm_distill_how {
+  int64_t rows, vocab;          /* of the logits; at most 2^24 rows */
+  int64_t ignore_index;         /* a row with this target does not count: loss and gradient zero, whatever its logits */
+  int32_t k;                    /* the teacher's entries of every row, at most 1024 */
+  int32_t dtype;                /* of the logits and their gradient */
+  int32_t index_dtype;          /* TDM_I64 or TDM_I32 */
+  int32_t teacher_dtype;
+  int32_t target_dtype;         /* TDM_I64 or TDM_I32 */
+  int32_t reduction;            /* of the rows that count (TDM_DISTILL_MEAN: their sum over their number, zero if there are none) */
+  float temperature, weight;    /* weight: the teacher's share, 0 to 1 */
+  float scale;                  /* of the gradient */
+} tdm_distill_how;
+
+/* For a row x of logits [rows, vocab], the teacher's logits t [rows, k] at the columns teacher_index [rows, k], temperature T,
+ * weight a and target y (targets [rows], NULL with weight 1: all rows count):
+ *
+ *     p = softmax(t / T),   row = a T^2 sum_k p_k (log p_k - log softmax(x / T)[index_k]) - (1 - a) log softmax(x)[y]
+ *
+ * loss (fp32: one value, or [rows] with TDM_DISTILL_NONE; NULL: not wanted) and grad [rows, vocab] (NULL: not wanted), the gradient
+ * of scale * upstream * loss with respect to the logits, rounded once. upstream (fp32 in GPU memory: one value, or [rows]
+ * with TDM_DISTILL_NONE) may be NULL: ones. With keep_ones the gradient of the rows whose upstream is 1 is left as it is: a caller that
+ * has it from an earlier call computes only what an upstream value changes. A teacher's entry with a negative column or a logit of
+ * -inf says nothing; a row without another has no first term; entries of the same column add up. A column, or a target that
+ * is used, outside the vocabulary and a NaN among the teacher's logits make the row's loss and gradient NaN; nothing is read there.
+ * logits is contiguous; grad starts at the same distance from a 16-byte boundary as logits. The workspace starts
+ * on 16 bytes and holds tdm_k7_distill_workspace(how) bytes (-1: arguments out of range). Sums have a fixed order. */
+int64_t tdm_k7_distill_workspace(const tdm_distill_how* how);
+int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* teacher_index, const void* teacher_logits, const void* targets,
+                   float* loss, void* grad, const float* upstream, int keep_ones, void* workspace, int64_t workspace_bytes, tdm_stream stream);
+
 /* ---- the engine: Group(backend="hip") --------------------------------------- */
 
 /* One rank's half of a group whose ranks are processes sharing one GPU. Mirrors

@@ -70,6 +70,12 @@ class QkShape(ctypes.Structure):
                 ("weight_dtype", ctypes.c_int32), ("position_dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
+class DistillHow(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("ignore_index", ctypes.c_int64), ("k", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("index_dtype", ctypes.c_int32), ("teacher_dtype", ctypes.c_int32), ("target_dtype", ctypes.c_int32),
+                ("reduction", ctypes.c_int32), ("temperature", ctypes.c_float), ("weight", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
 _PHEADS, _PSHAPE, _PPOSITIONS = ctypes.POINTER(HeadsView), ctypes.POINTER(QkShape), ctypes.POINTER(Positions)
 
 _SIGNATURES = {
@@ -138,6 +144,10 @@ _SIGNATURES = {
     "tdm_k6_qk_norm_rope_grad": (ctypes.c_int, [_PSHAPE, _PHEADS, _PHEADS, _PHEADS, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p,
                                                 _PPOSITIONS, ctypes.c_void_p, _PHEADS, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "tdm_k7_distill_workspace": (ctypes.c_int64, [ctypes.POINTER(DistillHow)]),
+    "tdm_k7_distill": (ctypes.c_int, [ctypes.POINTER(DistillHow), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
+                                      ctypes.c_void_p]),
 }
 
 _lib = None

@@ -16,7 +16,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libtandem_hip.so")
-SOURCES = ["kernels.hip", "kernels_chain.hip", "abi.hip", "engine.hip", "engine_abi.hip", "embedding.hip", "qk_rope.hip"]
+SOURCES = ["kernels.hip", "kernels_chain.hip", "abi.hip", "engine.hip", "engine_abi.hip", "embedding.hip", "qk_rope.hip", "distill.hip"]
 PROBE_LIB = os.path.join(CSRC, "libtandem_probe.so")
 PROBE_SOURCES = ["probe.hip"]
 

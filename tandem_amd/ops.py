@@ -1,5 +1,6 @@
 """The operators of the model that torch has no single pass for, as HIP kernels: the embedding lookup with a scale and its
-gradient by sorted tokens; the norms of queries and keys per head with the position rotation in the same pass.
+gradient by sorted tokens; the norms of queries and keys per head with the position rotation in the same pass;
+the distillation loss from a teacher's top logits with its gradient.
 
 Functions on tensors in GPU memory, differentiable, launched on the current stream of the tensors' device; float32,
 float16 and bfloat16, sums in fp32, one rounding at the end. Each has its gradient beside it (`*_grad`) for programs that
@@ -12,7 +13,7 @@ import ctypes
 
 import torch
 
-from ._lib import HeadsView, Positions, QkShape, check, dtype_code, lib, require_device_tensor, stream_ptr
+from ._lib import DistillHow, HeadsView, Positions, QkShape, check, dtype_code, lib, require_device_tensor, stream_ptr
 
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 INDEX_DTYPES = (torch.int64, torch.int32)
@@ -322,3 +323,105 @@ class _QkvNormRope(torch.autograd.Function):
         dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
         grads = _qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, ctx.how, *_split_qkv(dqkv, *ctx.heads))
         return (dqkv, None, None, *grads, None)
+
+
+# ---- distillation from a teacher's top logits
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def distill_loss(logits, teacher_index, teacher_logits, targets=None, temperature=1.0, weight=1.0, ignore_index=-100, reduction="mean"):
+    """The loss of a student's logits [..., vocab] against a teacher's k top logits teacher_logits [..., k] at the columns
+    teacher_index [..., k], mixed with the cross-entropy of hard targets [...]. For a row x, T the temperature, a the weight:
+
+        p = softmax(teacher_logits / T)
+        a T^2 sum_k p_k (log p_k - log softmax(x / T)[index_k]) + (1 - a) (-log softmax(x)[target])
+
+    averaged ("mean") or added up ("sum") over the rows that count, or one value per row ("none"), in fp32. A row whose target is
+    ignore_index does not count: its loss and gradient are zero, whatever its logits are; without any row that counts the mean is
+    zero. Targets may be given with weight 1 to say which rows count. An entry with a negative column or a teacher's logit of
+    -inf says nothing; a row without another takes no part in the first term; a column named twice has the sum of its
+    entries. A column, or a target that is used, outside the vocabulary and a NaN among the teacher's logits show: the row's loss
+    and gradient are NaN.
+
+    logits contiguous, float32, float16 or bfloat16; the teacher's logits any of these; k at most 1024. Where a gradient is needed
+    it is computed with the loss, from one reading of the logits, and kept until the backward pass hands it out. An upstream
+    gradient other than one (a loss that is scaled or divided afterwards) makes the backward pass compute it again."""
+    how, operands = _check_distill(logits, teacher_index, teacher_logits, targets, temperature, weight, ignore_index, reduction, 1.0)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Distill.apply(logits, *operands, how)
+    return _distill(logits, *operands, how, True, None, None, False)
+
+
+def distill_loss_and_grad(logits, teacher_index, teacher_logits, targets=None, temperature=1.0, weight=1.0, ignore_index=-100, reduction="mean",
+                          scale=1.0):
+    """(loss, gradient of scale * loss with respect to logits), for programs that run their backward pass by hand; the arguments are
+    distill_loss's. `scale`: what the loss is multiplied with before the gradient is rounded to the logits' type (loss scaling);
+    the loss that is returned is not scaled. With reduction "none" the gradient is that of the sum."""
+    how, operands = _check_distill(logits, teacher_index, teacher_logits, targets, temperature, weight, ignore_index, reduction, scale)
+    grad = _empty_at_phase_of(logits)
+    return _distill(logits, *operands, how, True, grad, None, False), grad
+
+
+def _empty_at_phase_of(t):
+    """An uninitialised contiguous tensor like `t` that starts at the same distance from a 16-byte boundary."""
+    lead = t.data_ptr() % 16 // t.element_size()
+    if lead == 0:
+        return torch.empty(t.shape, device=t.device, dtype=t.dtype)
+    return torch.empty(t.numel() + lead, device=t.device, dtype=t.dtype)[lead:].view(t.shape)
+
+
+def _check_distill(logits, index, teacher, targets, temperature, weight, ignore_index, reduction, scale):
+    _floating(logits, "distill_loss(logits)")
+    _floating(teacher, "distill_loss(teacher_logits)")
+    index = _indices(index, "distill_loss(teacher_index)")
+    if logits.dim() < 1 or logits.shape[-1] == 0 or teacher.dim() < 1 or teacher.shape[-1] == 0:
+        raise ValueError(f"logits {list(logits.shape)}, teacher_logits {list(teacher.shape)}: [..., vocab] and [..., k]")
+    if teacher.shape[:-1] != logits.shape[:-1] or index.shape != teacher.shape:
+        raise ValueError(f"logits {list(logits.shape)}, teacher_index {list(index.shape)}, teacher_logits {list(teacher.shape)}: rows differ")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction}")
+    if targets is not None:
+        targets = _indices(targets, "distill_loss(targets)")
+        if targets.shape != logits.shape[:-1]:
+            raise ValueError(f"targets {list(targets.shape)} for logits {list(logits.shape)}")
+    elif weight != 1.0:
+        raise ValueError("a weight below 1 needs targets")
+    _same_device(logits, index, teacher, targets)
+    vocab = logits.shape[-1]
+    how = DistillHow(logits.numel() // vocab, vocab, ignore_index, teacher.shape[-1], dtype_code(logits.dtype), dtype_code(index.dtype),
+                     dtype_code(teacher.dtype), dtype_code(torch.int64 if targets is None else targets.dtype), REDUCTIONS[reduction],
+                     temperature, weight, scale)
+    return how, (index, teacher, targets)
+
+
+def _distill(logits, index, teacher, targets, how, want_loss, grad, upstream, keep_ones):
+    L = lib()
+    need = L.tdm_k7_distill_workspace(how)
+    if need < 0:
+        raise ValueError(L.tdm_last_error().decode(errors="replace"))
+    work = torch.empty(need, device=logits.device, dtype=torch.uint8)
+    loss = torch.empty(logits.shape[:-1] if how.reduction == REDUCTIONS["none"] else (), device=logits.device) if want_loss else None
+    _call(logits.device, L.tdm_k7_distill, how, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), _ptr(targets), _ptr(loss), _ptr(grad),
+          _ptr(upstream), int(keep_ones), work.data_ptr(), need)
+    return loss
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, targets, how):
+        ctx.save_for_backward(logits, index, teacher, targets)
+        ctx.how, ctx.grad = how, _empty_at_phase_of(logits)
+        return _distill(logits, index, teacher, targets, how, True, ctx.grad, None, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, upstream):
+        # the gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out
+        # once; a second backward pass through the same graph computes its own.
+        grad, ctx.grad = ctx.grad, None
+        first = grad is not None
+        if not first:
+            grad = _empty_at_phase_of(ctx.saved_tensors[0])
+        _distill(*ctx.saved_tensors, ctx.how, False, grad, upstream.contiguous(), first)
+        return grad, None, None, None, None

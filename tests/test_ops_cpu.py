@@ -89,3 +89,44 @@ def test_qk_norm_rope_argument_errors_need_no_gpu():
     refused(grad(p, need - 1), "workspace")
     refused(grad(None, need), "workspace")
     refused(grad(ctypes.c_void_p(4100), need), "workspace")
+
+
+def test_distill_loss_refuses_cpu_tensors():
+    from tandem_amd import ops
+
+    with pytest.raises(ValueError, match="no CPU path"):
+        ops.distill_loss(torch.zeros(2, 8), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3))
+
+
+def test_distill_argument_errors_need_no_gpu():
+    lib = _lib()
+    L = lib.lib()
+    assert ctypes.sizeof(lib.DistillHow) == 64
+
+    def how(**change):
+        h = lib.DistillHow(4, 100, -100, 8, 0, 4, 0, 4, 1, 2.0, 1.0, 1.0)
+        for name, value in change.items():
+            setattr(h, name, value)
+        return h
+
+    p, off = ctypes.c_void_p(4096), ctypes.c_void_p(4100)  # never read
+    need = L.tdm_k7_distill_workspace(how())
+    assert need >= 16
+
+    def call(h, logits=p, index=p, targets=p, loss=p, grad=p, work=p, nbytes=need):
+        return L.tdm_k7_distill(h, logits, index, p, targets, loss, grad, None, 0, work, nbytes, None)
+
+    for change, word in ((dict(dtype=1), "logits"), (dict(teacher_dtype=4), "teacher"), (dict(index_dtype=0), "columns"), (dict(target_dtype=0), "targets"),
+                         (dict(rows=-1), "rows"), (dict(rows=(1 << 24) + 1), "rows"), (dict(vocab=0), "logits in a row"), (dict(vocab=1 << 31), "logits in a row"),
+                         (dict(k=0), "teacher's logits"), (dict(k=1025), "1024"), (dict(temperature=0.0), "temperature"),
+                         (dict(temperature=float("inf")), "temperature"), (dict(temperature=float("nan")), "temperature"), (dict(weight=-0.1), "weight"),
+                         (dict(weight=1.1), "weight"), (dict(weight=float("nan")), "weight"), (dict(reduction=3), "reduction")):
+        refused(call(how(**change)), word)
+        assert L.tdm_k7_distill_workspace(how(**change)) == -1
+    refused(call(how(weight=0.5), targets=None), "targets")
+    refused(call(how(), logits=None), "null")
+    refused(call(how(), index=None), "null")
+    refused(call(how(), loss=None, grad=None), "wanted")
+    refused(call(how(), nbytes=need - 1), "workspace")
+    refused(call(how(), work=off), "workspace")
+    refused(call(how(), grad=off), "16-byte")
