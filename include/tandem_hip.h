@@ -372,7 +372,7 @@ int tdm_k4_unit_gather_all(void* const* fulls, const void* const* shards, const 
  * pointer needs its element's alignment only, unless it says otherwise; what a launcher needs beyond its operands is a
  * workspace of the caller's, which it may fill with anything, and which two launches that can run at the same time must not share.
  *
- * out[i, :] = scale * weight[tokens[i], :] for i < n; weight [vocab, dim], out [n, dim], both contiguous. Tokens are
+ * out[i, :] = scale * weight[tokens[i], :] for i < n; weight [vocab, dim], out [n, dim], both contiguous; at most 2^28 tokens and 2^24 rows. Tokens are
  * TDM_I64 or TDM_I32 (index_dtype). A token outside [0, vocab) reads nothing; its row of out is NaN. */
 int tdm_k5_embedding(const void* weight, const void* tokens, int index_dtype, void* out, int64_t n, int64_t vocab, int64_t dim, int dtype,
                      float scale, tdm_stream stream);

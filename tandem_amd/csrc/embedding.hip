@@ -3,17 +3,15 @@
 //   out[n, :] = s * W[t_n, :]                      (one pass, a copy with a product)
 //   dW[v, :]  = s * sum over n with t_n = v of g[n, :],   in the order of n
 //
-// The gradient is a sum over rows that are strewn over g. The tokens are sorted first (stable, so that every row of dW
-// adds its terms in the order of n, run after run), then the rows of g are read once each, in sorted order, and added in
-// fp32 registers; a row of dW is written once, rounded once. No float atomics: the sums' order is fixed by n, the
-// vocabulary and the width alone.
+// The gradient is a sum over rows that are strewn over g. The tokens are brought together first (equal tokens side by side, in
+// the order of n), then the rows of g are read once each in that order and added in fp32 registers; a row of dW is written
+// once, rounded once. No float atomics: the order of every sum is fixed by n, the vocabulary and the width alone.
 //
-//   1. embedding_sort_kernel: a workgroup sorts a tile of tokens in LDS; the launch's other workgroups write the zeros of dW
-//      meanwhile (most rows of a large vocabulary get no token).
-//   2. embedding_merge_kernel (more than one tile): eight sorted runs become one, every entry finding its own place.
-//   3. embedding_sum_kernel: a wave takes a chunk of sorted entries and a slice of the columns. A token whose entries all lie in
-//      the chunk is finished there; one that crosses the chunk's ends leaves fp32 partial sums.
-//   4. embedding_join_kernel: adds the partial sums of the tokens that cross chunks, in order.
+//   1. embedding_sort_kernel: every workgroup reads all tokens and places those of its share of the vocabulary.
+//   2. embedding_sum_kernel: a wave takes a chunk of the sorted entries and a slice of the columns. A token whose entries all lie in
+//      the chunk is finished there; one that crosses the chunk's ends leaves fp32 partial sums. The launch's other workgroups
+//      write the zeros of the rows that have no token (most rows of a large vocabulary).
+//   3. embedding_join_kernel: adds the partial sums of the tokens that cross chunks, in order.
 
 #include <hip/hip_runtime.h>
 
@@ -75,207 +73,224 @@ __global__ __launch_bounds__(kLookupThreads) void embedding_lookup_kernel(Lookup
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr int kSortItems = 8;                             // per lane
-constexpr int kTile = kSortThreads * kSortItems;          // tokens that one workgroup sorts
-constexpr int kDigitBits = 9;
-constexpr int kDigits = 1 << kDigitBits;
-constexpr int kMergeWays = 8;
+constexpr int kMostShare = 512;  // tokens of the vocabulary that one workgroup places: a counter per wave and token in LDS
 
 struct SortArgs {
   const void* tokens;
-  uint32_t* keys;     // [n] sorted within every tile
-  uint32_t* order;    // [n] where the key came from
-  void* zero;         // dW
-  int64_t zero_bytes;
-  int64_t n, vocab, padding;
-  int tiles;
-  int passes, digit_bits;
+  uint32_t* keys;    // [entries] the sorted entries' tokens
+  uint32_t* order;   // [entries] where they came from
+  uint32_t* starts;  // [shares * share + 1] the first entry of every token, see place_of()
+  uint32_t vocab, padding;
+  uint32_t n, per_wave;  // per_wave: consecutive tokens that a wave reads, whole waves of lanes
+  uint32_t share;
+  int log_shares;
 };
 
-// The token as a sort key: a token that takes no gradient (outside the table, or the padding's) gets the key `vocab`, behind
-// all others.
-template <typename I>
-__device__ __forceinline__ uint32_t key_of(const SortArgs& a, int64_t n) {
-  const int64_t token = static_cast<int64_t>(static_cast<const I*>(a.tokens)[n]);
-  return static_cast<uint32_t>(token >= 0 && token < a.vocab && token != a.padding ? token : a.vocab);
+// Token v belongs to share v mod shares (neighbours, which occur together, are strewn) and is number v / shares in it; the
+// sorted order is that of this place.
+__host__ __device__ __forceinline__ uint32_t place_of(uint32_t v, uint32_t share, int log_shares) {
+  return (v & ((1u << log_shares) - 1)) * share + (v >> log_shares);
 }
 
-__device__ void write_zeros(char* base, int64_t bytes, int64_t block, int64_t blocks) {
-  typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
-  const int64_t head = std::min<int64_t>(bytes, (16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15);
-  const int64_t body = (bytes - head) / 16;
-  const vec16 none = {0u, 0u, 0u, 0u};
-  vec16* at = reinterpret_cast<vec16*>(base + head);
-  for (int64_t v = block * kSortThreads + threadIdx.x; v < body; v += blocks * kSortThreads) at[v] = none;
-  if (block == 0) {  // the bytes before the first and behind the last whole vector: whole elements of two bytes
-    const int64_t tail = (bytes - head - body * 16) / 2;
-    if (threadIdx.x < head / 2) reinterpret_cast<uint16_t*>(base)[threadIdx.x] = 0;
-    if (threadIdx.x < tail) reinterpret_cast<uint16_t*>(base + head + body * 16)[threadIdx.x] = 0;
-  }
+constexpr uint32_t kNoToken = 0xffffffffu;
+
+// A token that takes no gradient (outside the table, or the padding's) has no key and no entry.
+template <typename I>
+__device__ __forceinline__ uint32_t key_of(const SortArgs& a, uint32_t n) {
+  const I token = static_cast<const I*>(a.tokens)[n];
+  const uint32_t low = static_cast<uint32_t>(token);  // negative tokens: either the upper half is not zero or this exceeds any vocabulary
+  const bool fits = sizeof(I) == 4 || static_cast<uint32_t>(static_cast<uint64_t>(token) >> 32) == 0;
+  return fits && low < a.vocab && low != a.padding ? low : kNoToken;
 }
 
-// A tile by least significant digits, in LDS. A wave owns 512 consecutive entries, 64 at a time: the lanes with the same
-// digit find each other by ballots, the lowest of them moves the wave's count of that digit on, and an entry's rank is the
-// count it found there plus the lanes of its kind below it: stable, and the same every time.
-template <typename I>
+// Counting sort, a workgroup per share of the vocabulary. Every workgroup reads all tokens (they stay in L2): first it counts those
+// of lower shares and, per wave and token, those of its own; after a sum over tokens and waves it knows where each wave's entries
+// of each token go, and places them in the order in which they come: a wave walks its stretch of tokens 64 at a
+// time, and for every distinct token of its share among the 64 moves that token's counter on once. Any skew is right, and the
+// result is the same every time. A lane reads kHeld tokens at once; where they are all its tokens, they stay in registers for
+// the second walk. (A radix sort of 8192 tokens in one workgroup's LDS took 12.6 us for 8192 byte tokens, its
+// merge of four such tiles another 12: one compute unit's instruction rate bound it.)
+template <typename I, int kHeld>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a) {
-  if (static_cast<int>(blockIdx.x) >= a.tiles) {
-    write_zeros(static_cast<char*>(a.zero), a.zero_bytes, static_cast<int64_t>(blockIdx.x) - a.tiles, static_cast<int64_t>(gridDim.x) - a.tiles);
-    return;
-  }
-  __shared__ uint32_t s_key[kTile];
-  __shared__ uint16_t s_from[kTile];
-  __shared__ uint32_t s_count[kSortWaves][kDigits];
-  __shared__ uint32_t s_wave[kSortWaves];
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int here = static_cast<int>(std::min<int64_t>(kTile, a.n - base));
+  extern __shared__ uint32_t s_count[];  // [waves][share]
+  __shared__ uint32_t s_sum[kSortWaves], s_below[kSortWaves];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const uint32_t mine = blockIdx.x, low = (1u << a.log_shares) - 1;
+  uint32_t* const count = s_count + wave * a.share;
+  const uint32_t first = std::min<uint64_t>(static_cast<uint64_t>(wave) * a.per_wave, a.n);
+  const uint32_t end = std::min<uint64_t>(static_cast<uint64_t>(first) + a.per_wave, a.n);
+  uint32_t key[kHeld];
+  auto read = [&](uint32_t at) {
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const uint32_t n = at + u * kWave + lane;
+      key[u] = n < end ? key_of<I>(a, n) : kNoToken;
+    }
+  };
+  // a token's number in this share; kNoToken: it is another's
+  auto own = [&](uint32_t k) { return ((k ^ mine) & low) == 0 && k != kNoToken ? k >> a.log_shares : kNoToken; };
+  read(first);
+  for (uint32_t i = tid; i < kSortWaves * a.share; i += kSortThreads) s_count[i] = 0;
+  __syncthreads();
 
-  uint32_t key[kSortItems];
-  uint16_t from[kSortItems];
+  uint32_t below = 0;
+  for (uint32_t at = first; at < end; at += kWave * kHeld) {
+    if (at != first) read(at);
 #pragma unroll
-  for (int r = 0; r < kSortItems; ++r) {
-    const int e = wave * (kSortItems * kWave) + r * kWave + lane;
-    from[r] = static_cast<uint16_t>(e);
-    key[r] = e < here ? key_of<I>(a, base + e) : 0xffffffffu;  // behind everything in every pass: it stays last
+    for (int u = 0; u < kHeld; ++u) {
+      below += static_cast<uint32_t>(__popcll(__ballot((key[u] & low) < mine)));  // kNoToken is in no lower share
+      key[u] = own(key[u]);
+      if (key[u] != kNoToken) atomicAdd(&count[key[u]], 1u);
+    }
   }
-  const int digits = 1 << a.digit_bits;
-  for (int pass = 0; pass < a.passes; ++pass) {
-    const int shift = pass * a.digit_bits;
-    for (int i = tid; i < kSortWaves * kDigits; i += kSortThreads) (&s_count[0][0])[i] = 0;
-    __syncthreads();
-    uint32_t rank[kSortItems];
+  if (lane == 0) s_below[wave] = below;
+  __syncthreads();
+
+  uint32_t of_wave[kSortWaves] = {}, total = 0;
+  if (tid < a.share)
 #pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-      const uint32_t d = (key[r] >> shift) & (digits - 1);
-      uint64_t same = ~0ull;
-      for (int b = 0; b < a.digit_bits; ++b) {
-        const bool on = (d >> b) & 1;
-        const uint64_t votes = __ballot(on);
-        same &= on ? votes : ~votes;
+    for (int w = 0; w < kSortWaves; ++w) of_wave[w] = s_count[w * a.share + tid];
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) total += of_wave[w];
+  uint32_t upto = total;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint32_t x = __shfl_up(upto, d);
+    if (lane >= static_cast<uint32_t>(d)) upto += x;
+  }
+  if (lane == kWave - 1) s_sum[wave] = upto;
+  __syncthreads();
+  uint32_t begin = upto - total;
+#pragma unroll
+  for (uint32_t w = 0; w < kSortWaves; ++w) begin += s_below[w] + (w < wave ? s_sum[w] : 0u);
+  if (tid < a.share) {
+    a.starts[mine * a.share + tid] = begin;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      s_count[w * a.share + tid] = begin;
+      begin += of_wave[w];
+    }
+    if (mine == low && tid == a.share - 1) a.starts[(low + 1) * a.share] = begin;  // all entries
+  }
+  __syncthreads();
+
+  for (uint32_t at = first; at < end; at += kWave * kHeld) {
+    if (a.per_wave > kWave * kHeld) {
+      read(at);
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) key[u] = own(key[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      uint64_t left = __ballot(key[u] != kNoToken);
+      while (left != 0) {
+        const int leader = __builtin_ctzll(left);
+        const uint32_t k = __builtin_amdgcn_readlane(key[u], leader);
+        const uint64_t same = __ballot(key[u] == k);
+        uint32_t to = 0;
+        if (lane == static_cast<uint32_t>(leader)) to = atomicAdd(&count[k], static_cast<uint32_t>(__popcll(same)));
+        to = __builtin_amdgcn_readlane(to, leader);
+        if (key[u] == k) {
+          const uint32_t entry = to + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1)));
+          a.keys[entry] = (k << a.log_shares) | mine;
+          a.order[entry] = at + u * kWave + lane;
+        }
+        left &= ~same;
       }
-      const int leader = __ffsll(static_cast<unsigned long long>(same)) - 1;
-      uint32_t found = 0;
-      if (lane == leader) found = atomicAdd(&s_count[wave][d], static_cast<uint32_t>(__popcll(same)));
-      found = __shfl(found, leader);
-      rank[r] = found + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1)));
-    }
-    __syncthreads();
-    // where each wave's entries of each digit begin: an exclusive sum over digits, and over waves within a digit
-    uint32_t total = 0, mine = 0;
-    if (tid < digits)
-      for (int w = 0; w < kSortWaves; ++w) total += s_count[w][tid];
-    mine = total;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const uint32_t below = __shfl_up(mine, d);
-      if (lane >= d) mine += below;
-    }
-    if (lane == kWave - 1) s_wave[wave] = mine;
-    __syncthreads();
-    uint32_t begin = mine - total;
-    for (int w = 0; w < wave; ++w) begin += s_wave[w];
-    if (tid < digits)
-      for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = s_count[w][tid];
-        s_count[w][tid] = begin;
-        begin += c;
-      }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-      const uint32_t d = (key[r] >> shift) & (digits - 1);
-      const uint32_t to = s_count[wave][d] + rank[r];
-      s_key[to] = key[r];
-      s_from[to] = from[r];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSortItems; ++r) {
-      const int e = wave * (kSortItems * kWave) + r * kWave + lane;
-      key[r] = s_key[e];
-      from[r] = s_from[e];
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int r = 0; r < kSortItems; ++r) {
-    const int e = wave * (kSortItems * kWave) + r * kWave + lane;
-    if (e < here) {
-      a.keys[base + e] = key[r];
-      a.order[base + e] = static_cast<uint32_t>(base + from[r]);
     }
   }
-}
-
-// Eight sorted runs of `run` entries become one: an entry's place is its own index plus, for every other run of its group,
-// the number of that run's entries that go before it (equal keys of an earlier run do, of a later one do not: stable).
-struct MergeArgs {
-  const uint32_t *keys, *order;
-  uint32_t *to_keys, *to_order;
-  int64_t n, run;
-};
-
-__global__ __launch_bounds__(256) void embedding_merge_kernel(MergeArgs a) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= a.n) return;
-  const uint32_t key = a.keys[i];
-  const int64_t group = i / (a.run * kMergeWays) * (a.run * kMergeWays);
-  const int64_t own = (i - group) / a.run;
-  int64_t place = i - (group + own * a.run);
-  for (int r = 0; r < kMergeWays; ++r) {
-    if (r == own) continue;
-    const int64_t begin = group + r * a.run;
-    if (begin >= a.n) break;
-    int64_t lo = begin, hi = std::min<int64_t>(begin + a.run, a.n);
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      const uint32_t k = a.keys[mid];
-      if (r < own ? k <= key : k < key) lo = mid + 1;
-      else hi = mid;
-    }
-    place += lo - begin;
-  }
-  a.to_keys[group + place] = key;
-  a.to_order[group + place] = a.order[i];
 }
 
 // ---------------------------------------------------------------- sums
 
 constexpr int kSumWaves = 4;  // per workgroup
+constexpr int kSumThreads = kSumWaves * kWave;
+constexpr int kZeroBytes = 65536, kZeroRows = 1024;  // of dW, at most, per workgroup that writes zeros
 
 struct SumArgs {
   const void* grad;
-  const uint32_t *keys, *order;
+  const uint32_t *keys, *order, *starts;
   void* dweight;
-  float* partial;  // [chunks][2][dim]: of the token that the chunk begins inside of, of the token that it ends inside of
-  int64_t n, vocab, dim;
-  int chunk;   // entries
-  int slices;  // of a row
-  int vecs;    // accesses per row
+  float* partial;  // [chunks][2][pitch]: of the token that the chunk begins inside of, of the token that it ends inside of
+  int64_t vocab, dim, pitch;
+  uint32_t share;
+  int log_shares;
+  uint32_t all;       // place of the number of entries in `starts`
+  int chunk;          // entries
+  int slices;         // of a row
+  int vecs;           // accesses per row
+  uint32_t sums;      // workgroups that add; the others write zeros
+  int zero_rows;      // each
   float scale;
 };
 
 template <typename T, int kBytes>
-__global__ __launch_bounds__(kSumWaves * kWave) void embedding_sum_kernel(SumArgs a) {
+__device__ void zero_rows(const SumArgs& a) {
+  __shared__ uint8_t s_empty[kZeroRows];
+  const int64_t first = static_cast<int64_t>(blockIdx.x - a.sums) * a.zero_rows;
+  const int rows = static_cast<int>(std::min<int64_t>(a.zero_rows, a.vocab - first));
+  for (int r = threadIdx.x; r < rows; r += kSumThreads) {
+    const uint32_t p = place_of(static_cast<uint32_t>(first + r), a.share, a.log_shares);
+    s_empty[r] = a.starts[p] == a.starts[p + 1];
+  }
+  __syncthreads();
+  char* const to = static_cast<char*>(a.dweight) + first * a.dim * static_cast<int64_t>(sizeof(T));
+  typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
+  const vec16 none = {0u, 0u, 0u, 0u};
+  const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * static_cast<uint32_t>(sizeof(T));
+  const uint32_t bytes = static_cast<uint32_t>(rows) * row_bytes;
+  if (kBytes == 16 && a.vecs >= kWave) {  // a wave per row
+    for (int r = threadIdx.x / kWave; r < rows; r += kSumWaves) {
+      if (!s_empty[r]) continue;
+      char* const row = to + static_cast<int64_t>(r) * row_bytes;
+      for (uint32_t v = threadIdx.x % kWave; v < static_cast<uint32_t>(a.vecs); v += kWave) *reinterpret_cast<vec16*>(row + v * 16u) = none;
+    }
+    return;
+  }
+  // short rows, or rows that start anywhere: whole vectors over the ends of rows where all of their rows are empty
+  const uint32_t skip = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to) & 15);  // the first vector begins this far before the rows
+  for (uint32_t v = threadIdx.x; v * 16u < skip + bytes; v += kSumThreads) {
+    const uint32_t begin = v * 16u < skip ? 0u : v * 16u - skip, end = std::min(v * 16u + 16u - skip, bytes);
+    const uint32_t last = (end - 1) / row_bytes;
+    uint32_t row = begin / row_bytes;
+    bool all = end - begin == 16u;
+    for (uint32_t r = row; all && r <= last; ++r) all = s_empty[r];
+    if (all) {
+      *reinterpret_cast<vec16*>(to + begin) = none;
+      continue;
+    }
+    for (uint32_t b = begin; b < end; b += sizeof(T)) {
+      row = b / row_bytes;
+      if (s_empty[row]) *reinterpret_cast<T*>(to + b) = narrow<T>(0.0f);
+    }
+  }
+}
+
+template <typename T, int kBytes>
+__global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(SumArgs a) {
   constexpr int kN = kBytes / static_cast<int>(sizeof(T));
   constexpr int kAhead = 8;  // rows in flight
   using P = Pack<T, kN>;
+  if (blockIdx.x >= a.sums) {
+    zero_rows<T, kBytes>(a);
+    return;
+  }
   const int lane = threadIdx.x % kWave;
   const int64_t task = static_cast<int64_t>(blockIdx.x) * kSumWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t chunk = task / a.slices;
   const int64_t first = chunk * a.chunk;
-  if (first >= a.n) return;
+  const int64_t all = a.starts[a.all];
+  if (first >= all) return;
   const int vec = static_cast<int>(task % a.slices) * kWave + lane;
   const bool active = vec < a.vecs;
   const int64_t col = static_cast<int64_t>(active ? vec : 0) * kN;
-  const int count = static_cast<int>(std::min<int64_t>(a.chunk, a.n - first));
+  const int count = static_cast<int>(std::min<int64_t>(a.chunk, all - first));
 
-  const uint32_t none = static_cast<uint32_t>(a.vocab);
-  const uint32_t my_key = lane < count ? a.keys[first + lane] : none;
+  const uint32_t my_key = lane < count ? a.keys[first + lane] : kNoToken;
   const uint32_t my_row = lane < count ? a.order[first + lane] : 0u;
-  const uint32_t before = first > 0 ? a.keys[first - 1] : none;
-  const uint32_t after = first + count < a.n ? a.keys[first + count] : none;
+  const uint32_t before = first > 0 ? a.keys[first - 1] : kNoToken;
+  const uint32_t after = first + count < all ? a.keys[first + count] : kNoToken;
 
   float acc[kN];
 #pragma unroll
@@ -286,9 +301,14 @@ __global__ __launch_bounds__(kSumWaves * kWave) void embedding_sum_kernel(SumArg
   auto flush = [&](uint32_t k, bool began_before, bool goes_on) {
     if (!active) return;
     if (began_before || goes_on) {
-      float* to = a.partial + (chunk * 2 + (began_before ? 0 : 1)) * a.dim + col;
+      Pack<float, kN < 4 ? kN : 4> p;
+      float* to = a.partial + (chunk * 2 + (began_before ? 0 : 1)) * a.pitch + col;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) to[i] = acc[i];
+      for (int i = 0; i < kN; i += 4) {
+#pragma unroll
+        for (int j = 0; j < (kN < 4 ? kN : 4); ++j) p.v[j] = acc[i + j];
+        p.store(to + i);
+      }
     } else {
       P p;
 #pragma unroll
@@ -310,7 +330,7 @@ __global__ __launch_bounds__(kSumWaves * kWave) void embedding_sum_kernel(SumArg
       if (e + u < count) {
         const uint32_t k = __builtin_amdgcn_readlane(my_key, e + u);
         if (k != key) {
-          if (key != none) flush(key, open, false);
+          flush(key, open, false);
           key = k;
           open = false;
 #pragma unroll
@@ -321,47 +341,62 @@ __global__ __launch_bounds__(kSumWaves * kWave) void embedding_sum_kernel(SumArg
       }
     }
   }
-  if (key != none) flush(key, open, key == after);
+  flush(key, open, key == after);
 }
 
-// A workgroup per chunk and slice of 256 columns: if a token begins in the chunk and goes on behind it, its partial sums.
-constexpr int kJoinThreads = 256;
+// A workgroup per chunk and slice of 256 columns: if a token begins in the chunk and goes on behind it, its partial sums, the
+// workgroup's four waves a quarter of them each.
+constexpr int kJoinWaves = 4;
+constexpr int kJoinCols = 4 * kWave;
 
 template <typename T>
-__global__ __launch_bounds__(kJoinThreads) void embedding_join_kernel(SumArgs a) {
+__global__ __launch_bounds__(kJoinWaves* kWave) void embedding_join_kernel(SumArgs a) {
+  __shared__ float s_acc[kJoinWaves][kJoinCols];
   const int64_t chunk = blockIdx.x;
   const int64_t first = chunk * a.chunk, next = first + a.chunk;
-  if (next >= a.n) return;
+  if (next >= a.starts[a.all]) return;
   const uint32_t key = a.keys[next - 1];
-  if (key == static_cast<uint32_t>(a.vocab) || a.keys[next] != key) return;
-  if (first > 0 && a.keys[first] == key && a.keys[first - 1] == key) return;  // it began earlier
-  int64_t lo = next, hi = a.n;  // the first entry behind the token's last
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (a.keys[mid] <= key) lo = mid + 1;
-    else hi = mid;
-  }
-  const int64_t last = (lo - 1) / a.chunk;
-  const int64_t col = static_cast<int64_t>(blockIdx.y) * kJoinThreads + threadIdx.x;
-  if (col >= a.dim) return;
-  float acc = a.partial[(chunk * 2 + 1) * a.dim + col];
+  const uint32_t place = place_of(key, a.share, a.log_shares);
+  const int64_t begin = a.starts[place], end = a.starts[place + 1];
+  if (begin < first || end <= next) return;  // it began earlier, or ends here
+  const int64_t heads = (end - 1) / a.chunk - chunk;  // chunks behind this one that it reaches into
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int64_t col = static_cast<int64_t>(blockIdx.y) * kJoinCols + lane * 4;
+  const int64_t per = (heads + kJoinWaves - 1) / kJoinWaves;
+  const int64_t from = chunk + 1 + wave * per, to = std::min(chunk + 1 + heads, from + per);
+  using P4 = Pack<float, 4>;
+  P4 acc{};
+  if (col < a.dim) {
+    if (wave == 0) acc = P4::load(a.partial + (chunk * 2 + 1) * a.pitch + col);
 #pragma unroll 8
-  for (int64_t c = chunk + 1; c <= last; ++c) acc += a.partial[c * 2 * a.dim + col];
-  static_cast<T*>(a.dweight)[static_cast<int64_t>(key) * a.dim + col] = narrow<T>(acc * a.scale);
+    for (int64_t c = from; c < to; ++c) {
+      const P4 p = P4::load(a.partial + c * 2 * a.pitch + col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc.v[i] += p.v[i];
+    }
+  }
+  acc.store(&s_acc[wave][lane * 4]);
+  __syncthreads();
+  const int64_t c = static_cast<int64_t>(blockIdx.y) * kJoinCols + threadIdx.x;
+  if (c >= a.dim) return;
+  float sum = s_acc[0][threadIdx.x];
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) sum += s_acc[w][threadIdx.x];
+  static_cast<T*>(a.dweight)[static_cast<int64_t>(key) * a.dim + c] = narrow<T>(sum * a.scale);
 }
 
 // ---------------------------------------------------------------- host
 
 constexpr int64_t kMostTokens = int64_t(1) << 28;  // the sums' launch stays below 2^32 lanes
 
-int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+constexpr int64_t kMostVocab = int64_t(1) << 24;  // 2^14 workgroups place the tokens
 
 int chunk_of(int64_t n) { return n <= 16384 ? 16 : n <= 65536 ? 32 : 64; }
 
 void check_shape(int64_t n, int64_t vocab, int64_t dim, int dtype) {
   require(operator_dtype(dtype), "embedding: the dtype must be float32, float16 or bfloat16");
   require(n >= 0 && n <= kMostTokens, "embedding: 0 to 2^28 tokens");
-  require(vocab >= 1 && vocab < (int64_t(1) << 31), "embedding: a vocabulary of 1 to 2^31 - 1 rows");
+  require(vocab >= 1 && vocab <= kMostVocab, "embedding: a vocabulary of 1 to 2^24 rows");
   require(dim >= 1 && dim <= (int64_t(1) << 20), "embedding: rows of 1 to 2^20 elements");
 }
 
@@ -379,24 +414,34 @@ void with_width(int width, F&& f) {
   }
 }
 
+// 64 shares, or as many more as it takes to keep a share's counters in LDS.
+int log_shares_of(int64_t vocab) {
+  int log = 6;
+  while (((vocab - 1) >> log) >= kMostShare) ++log;
+  return log;
+}
+
 struct Workspace {  // of the gradient
-  int64_t keys[2], order[2], partial, bytes;
+  int64_t keys, order, starts, partial, bytes;
+  int log_shares;
+  int64_t share, pitch;
 };
 
-Workspace workspace_of(int64_t n, int64_t dim) {
+Workspace workspace_of(int64_t n, int64_t vocab, int64_t dim) {
   Workspace w{};
   auto take = [&](int64_t bytes) {
     const int64_t at = w.bytes;
     w.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  const int sides = n > kTile ? 2 : 1;
-  for (int i = 0; i < sides; ++i) {
-    w.keys[i] = take(n * 4);
-    w.order[i] = take(n * 4);
-  }
+  w.log_shares = log_shares_of(vocab);
+  w.share = ((vocab - 1) >> w.log_shares) + 1;
+  w.pitch = (dim + 3) / 4 * 4;
+  w.keys = take(n * 4);
+  w.order = take(n * 4);
+  w.starts = take(((w.share << w.log_shares) + 1) * 4);
   const int64_t chunks = (n + chunk_of(n) - 1) / chunk_of(n);
-  w.partial = take(chunks > 1 ? chunks * 2 * dim * 4 : 0);
+  w.partial = take(chunks > 1 ? chunks * 2 * w.pitch * 4 : 0);
   return w;
 }
 
@@ -442,7 +487,7 @@ int64_t tdm_k5_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t dim) {
   int64_t bytes = -1;
   guard([&] {
     check_shape(n, vocab, dim, TDM_F32);
-    bytes = workspace_of(n, dim).bytes;
+    bytes = workspace_of(n, vocab, dim).bytes;
   });
   return bytes;
 }
@@ -453,8 +498,8 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     check_shape(n, vocab, dim, dtype);
     check_index(index_dtype);
     require(dweight != nullptr && (n == 0 || (grad != nullptr && tokens != nullptr)), "embedding_grad: null pointer");
-    const Workspace ws = workspace_of(n, dim);
-    require(n == 0 || (workspace != nullptr && workspace_bytes >= ws.bytes), "embedding_grad: the workspace is smaller than tdm_k5_embedding_grad_workspace says");
+    const Workspace ws = workspace_of(n, vocab, dim);
+    require(workspace != nullptr && workspace_bytes >= ws.bytes, "embedding_grad: the workspace is smaller than tdm_k5_embedding_grad_workspace says");
     require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "embedding_grad: the workspace must start on 16 bytes");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* const base = static_cast<char*>(workspace);
@@ -462,63 +507,62 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
 
     SortArgs s{};
     s.tokens = tokens;
-    s.zero = dweight;
-    s.zero_bytes = vocab * dim * es;
-    s.n = n;
-    s.vocab = vocab;
-    s.padding = padding;
-    s.tiles = static_cast<int>(tiles_of(n));
-    if (n > 0) {
-      s.keys = reinterpret_cast<uint32_t*>(base + ws.keys[0]);
-      s.order = reinterpret_cast<uint32_t*>(base + ws.order[0]);
-    }
-    int bits = 1;
-    while ((vocab >> bits) != 0) ++bits;  // keys are 0..vocab
-    s.passes = (bits + kDigitBits - 1) / kDigitBits;
-    s.digit_bits = (bits + s.passes - 1) / s.passes;
-    const int64_t fill = std::min<int64_t>((s.zero_bytes + 65535) / 65536, 2048);
-    const dim3 grid(static_cast<unsigned>(s.tiles + fill));
-    if (index_dtype == TDM_I64) hipLaunchKernelGGL((embedding_sort_kernel<int64_t>), grid, dim3(kSortThreads), 0, st, s);
-    else hipLaunchKernelGGL((embedding_sort_kernel<int32_t>), grid, dim3(kSortThreads), 0, st, s);
+    s.keys = reinterpret_cast<uint32_t*>(base + ws.keys);
+    s.order = reinterpret_cast<uint32_t*>(base + ws.order);
+    s.starts = reinterpret_cast<uint32_t*>(base + ws.starts);
+    s.vocab = static_cast<uint32_t>(vocab);
+    s.padding = padding >= 0 && padding < vocab ? static_cast<uint32_t>(padding) : kNoToken;
+    s.n = static_cast<uint32_t>(n);
+    s.per_wave = static_cast<uint32_t>((n + kSortThreads - 1) / kSortThreads * kWave);
+    s.share = static_cast<uint32_t>(ws.share);
+    s.log_shares = ws.log_shares;
+    const dim3 shares(1u << ws.log_shares);
+    const unsigned lds = kSortWaves * s.share * 4;
+    const int held = static_cast<int>(s.per_wave / kWave);
+    auto sort = [&](auto h) {
+      if (index_dtype == TDM_I64) hipLaunchKernelGGL((embedding_sort_kernel<int64_t, h.value>), shares, dim3(kSortThreads), lds, st, s);
+      else hipLaunchKernelGGL((embedding_sort_kernel<int32_t, h.value>), shares, dim3(kSortThreads), lds, st, s);
+    };
+    if (held <= 4) sort(std::integral_constant<int, 4>{});
+    else if (held <= 8) sort(std::integral_constant<int, 8>{});
+    else if (held <= 16) sort(std::integral_constant<int, 16>{});
+    else sort(std::integral_constant<int, 32>{});
     check_launch("embedding_sort launch");
-    if (n == 0) return;
-
-    int side = 0;
-    for (int64_t run = kTile; run < n; run *= kMergeWays) {
-      MergeArgs m{reinterpret_cast<uint32_t*>(base + ws.keys[side]), reinterpret_cast<uint32_t*>(base + ws.order[side]),
-                  reinterpret_cast<uint32_t*>(base + ws.keys[side ^ 1]), reinterpret_cast<uint32_t*>(base + ws.order[side ^ 1]), n, run};
-      hipLaunchKernelGGL(embedding_merge_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, st, m);
-      check_launch("embedding_merge launch");
-      side ^= 1;
-    }
 
     const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
     SumArgs a{};
     a.grad = grad;
-    a.keys = reinterpret_cast<uint32_t*>(base + ws.keys[side]);
-    a.order = reinterpret_cast<uint32_t*>(base + ws.order[side]);
+    a.keys = s.keys;
+    a.order = s.order;
+    a.starts = s.starts;
     a.dweight = dweight;
     a.partial = reinterpret_cast<float*>(base + ws.partial);
-    a.n = n;
     a.vocab = vocab;
     a.dim = dim;
+    a.pitch = ws.pitch;
+    a.share = s.share;
+    a.log_shares = s.log_shares;
+    a.all = s.share << s.log_shares;
     a.chunk = chunk_of(n);
     a.vecs = static_cast<int>(dim * es / width);
     a.slices = (a.vecs + kWave - 1) / kWave;
+    a.zero_rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kZeroRows, kZeroBytes / (dim * es))));
     a.scale = scale;
     const int64_t chunks = (n + a.chunk - 1) / a.chunk;
-    const int64_t groups = (chunks * a.slices + kSumWaves - 1) / kSumWaves;
-    require(groups <= (int64_t(1) << 24), "embedding_grad: more than 2^26 chunks and slices");
+    const int64_t sums = (chunks * a.slices + kSumWaves - 1) / kSumWaves;
+    const int64_t zeros = (vocab + a.zero_rows - 1) / a.zero_rows;
+    require(sums + zeros < (int64_t(1) << 24), "embedding_grad: too many tokens, rows or columns for one launch");
+    a.sums = static_cast<uint32_t>(sums);
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       with_width(width, [&](auto w) {
         if constexpr (w.value >= static_cast<int>(sizeof(T)))
-          hipLaunchKernelGGL((embedding_sum_kernel<T, w.value>), dim3(static_cast<unsigned>(groups)), dim3(kSumWaves * kWave), 0, st, a);
+          hipLaunchKernelGGL((embedding_sum_kernel<T, w.value>), dim3(static_cast<unsigned>(sums + zeros)), dim3(kSumThreads), 0, st, a);
       });
       check_launch("embedding_sum launch");
       if (chunks > 1) {
-        hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(static_cast<unsigned>(chunks), static_cast<unsigned>((dim + kJoinThreads - 1) / kJoinThreads)),
-                           dim3(kJoinThreads), 0, st, a);
+        hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(static_cast<unsigned>(chunks), static_cast<unsigned>((dim + kJoinCols - 1) / kJoinCols)),
+                           dim3(kJoinWaves * kWave), 0, st, a);
         check_launch("embedding_join launch");
       }
     });
