@@ -30,6 +30,7 @@ namespace {
 // ---------------------------------------------------------------- lookup
 
 constexpr int kLookupThreads = 256;
+constexpr int kLookupRows = 4;  // in flight at once
 
 struct LookupArgs {
   const void* weight;
@@ -47,24 +48,31 @@ __global__ __launch_bounds__(kLookupThreads) void embedding_lookup_kernel(Lookup
   using P = Pack<T, kN>;
   const int lanes = 1 << a.log_lanes;
   const int lane = threadIdx.x & (lanes - 1);
-  const int rows = kLookupThreads >> a.log_lanes;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * rows;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows + (threadIdx.x >> a.log_lanes); row < a.n; row += step) {
-    const int64_t token = static_cast<int64_t>(static_cast<const I*>(a.tokens)[row]);
-    const bool known = token >= 0 && token < a.vocab;
-    const T* from = static_cast<const T*>(a.weight) + (known ? token * a.dim : 0);
-    T* to = static_cast<T*>(a.out) + row * a.dim;
+  const int rows = kLookupThreads >> a.log_lanes;  // side by side
+  const int64_t step = static_cast<int64_t>(gridDim.x) * rows * kLookupRows;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * rows * kLookupRows + (threadIdx.x >> a.log_lanes); base < a.n; base += step) {
+    int64_t token[kLookupRows];
+#pragma unroll
+    for (int r = 0; r < kLookupRows; ++r) {
+      const int64_t row = base + r * rows;
+      token[r] = row < a.n ? static_cast<int64_t>(static_cast<const I*>(a.tokens)[row]) : 0;
+    }
     for (int v = lane; v < a.vecs; v += lanes) {
-      P p;
-      if (known) {
-        p = P::load(from + static_cast<int64_t>(v) * kN);
+      P p[kLookupRows];
 #pragma unroll
-        for (int i = 0; i < kN; ++i) p.v[i] = narrow<T>(widen(p.v[i]) * a.scale);
-      } else {  // a token outside the table reads nothing, and shows
-#pragma unroll
-        for (int i = 0; i < kN; ++i) p.v[i] = narrow<T>(__builtin_nanf(""));
+      for (int r = 0; r < kLookupRows; ++r) {
+        const bool known = token[r] >= 0 && token[r] < a.vocab;  // a token outside the table reads row 0, and shows
+        p[r] = P::load(static_cast<const T*>(a.weight) + (known ? token[r] * a.dim : 0) + static_cast<int64_t>(v) * kN);
       }
-      p.store(to + static_cast<int64_t>(v) * kN);
+#pragma unroll
+      for (int r = 0; r < kLookupRows; ++r) {
+        const int64_t row = base + r * rows;
+        const bool known = token[r] >= 0 && token[r] < a.vocab;
+        const float scale = known ? a.scale : __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < kN; ++i) p[r].v[i] = narrow<T>(widen(p[r].v[i]) * scale);
+        if (row < a.n) p[r].store_nt(static_cast<T*>(a.out) + row * a.dim + static_cast<int64_t>(v) * kN);
+      }
     }
   }
 }
@@ -84,6 +92,8 @@ struct SortArgs {
   uint32_t n, per_wave;  // per_wave: consecutive tokens that a wave reads, whole waves of lanes
   uint32_t share;
   int log_shares;
+  void* zero;          // the first bytes of dW, which the launch's other workgroups clear
+  int64_t zero_bytes;  // whole vectors from a 16-byte boundary on
 };
 
 // Token v belongs to share v mod shares (neighbours, which occur together, are strewn) and is number v / shares in it; the
@@ -111,7 +121,15 @@ __device__ __forceinline__ uint32_t key_of(const SortArgs& a, uint32_t n) {
 // the second walk. (A radix sort of 8192 tokens in one workgroup's LDS took 12.6 us for 8192 byte tokens, its
 // merge of four such tiles another 12: one compute unit's instruction rate bound it.)
 template <typename I, int kHeld>
-__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a) {
+__global__ __launch_bounds__(kSortThreads, 8) void embedding_sort_kernel(SortArgs a) {
+  if (blockIdx.x >> a.log_shares != 0) {
+    typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
+    const vec16 none = {0u, 0u, 0u, 0u};
+    vec16* const to = static_cast<vec16*>(a.zero);
+    const int64_t blocks = static_cast<int64_t>(gridDim.x) - (int64_t(1) << a.log_shares);
+    for (int64_t v = (blockIdx.x - (int64_t(1) << a.log_shares)) * kSortThreads + threadIdx.x; v < a.zero_bytes / 16; v += blocks * kSortThreads) __builtin_nontemporal_store(none, to + v);
+    return;
+  }
   extern __shared__ uint32_t s_count[];  // [waves][share]
   __shared__ uint32_t s_sum[kSortWaves], s_below[kSortWaves];
   const uint32_t tid = threadIdx.x, lane = tid % kWave;
@@ -181,22 +199,35 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) key[u] = own(key[u]);
     }
+    // the counters' answers of four steps are on their way at once: a wave's LDS operations stay in order
+    constexpr int kGroup = 4;
 #pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-      uint64_t left = __ballot(key[u] != kNoToken);
-      while (left != 0) {
-        const int leader = __builtin_ctzll(left);
-        const uint32_t k = __builtin_amdgcn_readlane(key[u], leader);
-        const uint64_t same = __ballot(key[u] == k);
-        uint32_t to = 0;
-        if (lane == static_cast<uint32_t>(leader)) to = atomicAdd(&count[k], static_cast<uint32_t>(__popcll(same)));
-        to = __builtin_amdgcn_readlane(to, leader);
-        if (key[u] == k) {
-          const uint32_t entry = to + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1)));
-          a.keys[entry] = (k << a.log_shares) | mine;
-          a.order[entry] = at + u * kWave + lane;
+    for (int v = 0; v < kHeld; v += kGroup) {
+      uint32_t found[kGroup], lead[kGroup], rank[kGroup];
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) {
+        found[u] = lead[u] = rank[u] = 0;
+        uint64_t left = __ballot(key[v + u] != kNoToken);
+        while (left != 0) {
+          const uint32_t leader = static_cast<uint32_t>(__builtin_ctzll(left));
+          const uint32_t k = __builtin_amdgcn_readlane(key[v + u], leader);
+          const bool same = key[v + u] == k;
+          const uint64_t all = __ballot(same);
+          if (same) {
+            lead[u] = leader;
+            rank[u] = static_cast<uint32_t>(__popcll(all & ((1ull << lane) - 1)));
+          }
+          if (lane == leader) found[u] = atomicAdd(&count[k], static_cast<uint32_t>(__popcll(all)));
+          left &= ~all;
         }
-        left &= ~same;
+      }
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) {
+        const uint32_t entry = __shfl(found[u], static_cast<int>(lead[u])) + rank[u];
+        if (key[v + u] != kNoToken) {
+          a.keys[entry] = (key[v + u] << a.log_shares) | mine;
+          a.order[entry] = at + (v + u) * kWave + lane;
+        }
       }
     }
   }
@@ -206,7 +237,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(SortArgs a
 
 constexpr int kSumWaves = 4;  // per workgroup
 constexpr int kSumThreads = kSumWaves * kWave;
-constexpr int kZeroBytes = 65536, kZeroRows = 1024;  // of dW, at most, per workgroup that writes zeros
+constexpr int64_t kHiddenBytes = int64_t(48) << 20, kHiddenPerToken = 1536;  // of zeros that the sort's launch writes
+constexpr int kZeroBytes = 16384, kZeroRows = 1024;  // of dW, at most, per workgroup that writes zeros
 
 struct SumArgs {
   const void* grad;
@@ -221,14 +253,15 @@ struct SumArgs {
   int slices;         // of a row
   int vecs;           // accesses per row
   uint32_t sums;      // workgroups that add; the others write zeros
-  int zero_rows;      // each
+  int64_t zero_from;  // the first row whose zeros are still to be written
+  int zero_rows;      // of each workgroup
   float scale;
 };
 
 template <typename T, int kBytes>
 __device__ void zero_rows(const SumArgs& a) {
   __shared__ uint8_t s_empty[kZeroRows];
-  const int64_t first = static_cast<int64_t>(blockIdx.x - a.sums) * a.zero_rows;
+  const int64_t first = a.zero_from + static_cast<int64_t>(blockIdx.x - a.sums) * a.zero_rows;
   const int rows = static_cast<int>(std::min<int64_t>(a.zero_rows, a.vocab - first));
   for (int r = threadIdx.x; r < rows; r += kSumThreads) {
     const uint32_t p = place_of(static_cast<uint32_t>(first + r), a.share, a.log_shares);
@@ -244,7 +277,7 @@ __device__ void zero_rows(const SumArgs& a) {
     for (int r = threadIdx.x / kWave; r < rows; r += kSumWaves) {
       if (!s_empty[r]) continue;
       char* const row = to + static_cast<int64_t>(r) * row_bytes;
-      for (uint32_t v = threadIdx.x % kWave; v < static_cast<uint32_t>(a.vecs); v += kWave) *reinterpret_cast<vec16*>(row + v * 16u) = none;
+      for (uint32_t v = threadIdx.x % kWave; v < static_cast<uint32_t>(a.vecs); v += kWave) __builtin_nontemporal_store(none, reinterpret_cast<vec16*>(row + v * 16u));
     }
     return;
   }
@@ -354,8 +387,9 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void embedding_join_kernel(SumAr
   __shared__ float s_acc[kJoinWaves][kJoinCols];
   const int64_t chunk = blockIdx.x;
   const int64_t first = chunk * a.chunk, next = first + a.chunk;
-  if (next >= a.starts[a.all]) return;
-  const uint32_t key = a.keys[next - 1];
+  const int64_t all = a.starts[a.all];
+  const uint32_t key = a.keys[next - 1];  // next is at most n; an entry behind the last holds anything
+  if (next >= all) return;
   const uint32_t place = place_of(key, a.share, a.log_shares);
   const int64_t begin = a.starts[place], end = a.starts[place + 1];
   if (begin < first || end <= next) return;  // it began earlier, or ends here
@@ -391,7 +425,12 @@ constexpr int64_t kMostTokens = int64_t(1) << 28;  // the sums' launch stays bel
 
 constexpr int64_t kMostVocab = int64_t(1) << 24;  // 2^14 workgroups place the tokens
 
-int chunk_of(int64_t n) { return n <= 16384 ? 16 : n <= 65536 ? 32 : 64; }
+// Entries of a chunk: 64, or fewer as long as there are fewer than 2048 waves of 512 columns.
+int chunk_of(int64_t n, int64_t dim) {
+  int chunk = 64;
+  while (chunk > 8 && n / chunk * ((dim + 511) / 512) < 2048) chunk /= 2;
+  return chunk;
+}
 
 void check_shape(int64_t n, int64_t vocab, int64_t dim, int dtype) {
   require(operator_dtype(dtype), "embedding: the dtype must be float32, float16 or bfloat16");
@@ -440,7 +479,8 @@ Workspace workspace_of(int64_t n, int64_t vocab, int64_t dim) {
   w.keys = take(n * 4);
   w.order = take(n * 4);
   w.starts = take(((w.share << w.log_shares) + 1) * 4);
-  const int64_t chunks = (n + chunk_of(n) - 1) / chunk_of(n);
+  const int chunk = chunk_of(n, dim);
+  const int64_t chunks = (n + chunk - 1) / chunk;
   w.partial = take(chunks > 1 ? chunks * 2 * w.pitch * 4 : 0);
   return w;
 }
@@ -466,7 +506,7 @@ int tdm_k5_embedding(const void* weight, const void* tokens, int index_dtype, vo
     const int width = access_width(reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(dim * es), es);
     LookupArgs a{weight, tokens, out, n, vocab, dim, static_cast<int>(dim * es / width), 0, scale};
     while ((1 << a.log_lanes) < a.vecs && (1 << a.log_lanes) < kLookupThreads) ++a.log_lanes;
-    const int rows = kLookupThreads >> a.log_lanes;
+    const int rows = (kLookupThreads >> a.log_lanes) * kLookupRows;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + rows - 1) / rows, int64_t(1) << 22)));
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
@@ -516,7 +556,15 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     s.per_wave = static_cast<uint32_t>((n + kSortThreads - 1) / kSortThreads * kWave);
     s.share = static_cast<uint32_t>(ws.share);
     s.log_shares = ws.log_shares;
-    const dim3 shares(1u << ws.log_shares);
+    // The sort leaves the memory idle: its launch clears as many rows as are written in about its time, whether they get
+    // a token or not. They begin on a vector and end with a row.
+    const int64_t row_bytes = dim * es;
+    int64_t hidden = std::min(vocab, (kHiddenBytes + n * kHiddenPerToken) / row_bytes);
+    if (reinterpret_cast<uintptr_t>(dweight) % 16 != 0) hidden = 0;
+    while (hidden * row_bytes % 16 != 0) --hidden;
+    s.zero = dweight;
+    s.zero_bytes = hidden * row_bytes;
+    const dim3 shares((1u << ws.log_shares) + static_cast<unsigned>(std::min<int64_t>((s.zero_bytes + 65535) / 65536, 1024)));
     const unsigned lds = kSortWaves * s.share * 4;
     const int held = static_cast<int>(s.per_wave / kWave);
     auto sort = [&](auto h) {
@@ -525,8 +573,7 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     };
     if (held <= 4) sort(std::integral_constant<int, 4>{});
     else if (held <= 8) sort(std::integral_constant<int, 8>{});
-    else if (held <= 16) sort(std::integral_constant<int, 16>{});
-    else sort(std::integral_constant<int, 32>{});
+    else sort(std::integral_constant<int, 16>{});
     check_launch("embedding_sort launch");
 
     const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
@@ -543,16 +590,18 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     a.share = s.share;
     a.log_shares = s.log_shares;
     a.all = s.share << s.log_shares;
-    a.chunk = chunk_of(n);
+    a.chunk = chunk_of(n, dim);
     a.vecs = static_cast<int>(dim * es / width);
     a.slices = (a.vecs + kWave - 1) / kWave;
-    a.zero_rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kZeroRows, kZeroBytes / (dim * es))));
+    a.zero_from = hidden;
+    a.zero_rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kZeroRows, kZeroBytes / row_bytes)));
     a.scale = scale;
     const int64_t chunks = (n + a.chunk - 1) / a.chunk;
     const int64_t sums = (chunks * a.slices + kSumWaves - 1) / kSumWaves;
-    const int64_t zeros = (vocab + a.zero_rows - 1) / a.zero_rows;
+    const int64_t zeros = (vocab - hidden + a.zero_rows - 1) / a.zero_rows;
     require(sums + zeros < (int64_t(1) << 24), "embedding_grad: too many tokens, rows or columns for one launch");
     a.sums = static_cast<uint32_t>(sums);
+    if (sums + zeros == 0) return;
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       with_width(width, [&](auto w) {
@@ -561,7 +610,7 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
       });
       check_launch("embedding_sum launch");
       if (chunks > 1) {
-        hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(static_cast<unsigned>(chunks), static_cast<unsigned>((dim + kJoinCols - 1) / kJoinCols)),
+        hipLaunchKernelGGL((embedding_join_kernel<T>), dim3(static_cast<unsigned>(n / a.chunk), static_cast<unsigned>((dim + kJoinCols - 1) / kJoinCols)),
                            dim3(kJoinWaves * kWave), 0, st, a);
         check_launch("embedding_join launch");
       }
