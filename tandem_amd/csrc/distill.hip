@@ -43,24 +43,6 @@ struct DistillArgs {
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ln_of(float x) { return __builtin_amdgcn_logf(x) * kLn2; }
 
-// Sum or maximum over the kG lanes of a row; every lane gets it. `s`: kG / 64 floats of LDS that nothing else uses.
-template <int kG, class F>
-__device__ __forceinline__ float over_row(float x, float* s, F f) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) x = f(x, __shfl_xor(x, d));
-  if constexpr (kG > kWave) {
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = x;
-    __syncthreads();
-    x = s[0];
-#pragma unroll
-    for (int w = 1; w < kG / kWave; ++w) x = f(x, s[w]);
-  }
-  return x;
-}
-struct Add { __device__ float operator()(float a, float b) const { return a + b; } };
-struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-
 __device__ __forceinline__ float teacher_logit(const DistillArgs& a, int64_t at) {
   if (a.teacher_dtype == TDM_F32) return static_cast<const float*>(a.teacher)[at];
   if (a.teacher_dtype == TDM_F16) return static_cast<float>(static_cast<const _Float16*>(a.teacher)[at]);
@@ -71,185 +53,337 @@ __device__ __forceinline__ int64_t index_of(const void* p, int i64, int64_t at) 
   return i64 ? static_cast<const int64_t*>(p)[at] : static_cast<int64_t>(static_cast<const int32_t*>(p)[at]);
 }
 
-// A workgroup of kG lanes per row. kMix: both temperatures are needed (a < 1 and T != 1).
-// LDS: kG / 64 floats, then k + 1 columns and k + 1 values.
-template <typename T, int kG, bool kMix>
-__global__ __launch_bounds__(kG) void distill_kernel(DistillArgs a) {
+// Where a row's whole vectors lie: `head` elements before them, `tail` behind. The gradient's row lies at the same phase.
+struct Body {
+  int head, vecs, tail;
+};
+template <typename T>
+__device__ __forceinline__ Body body_of(const T* x, int64_t vocab) {
   constexpr int kN = 16 / static_cast<int>(sizeof(T));
-  using P = Pack<T, kN>;
-  extern __shared__ float lds[];
-  float* const s_red = lds;
-  int32_t* const s_col = reinterpret_cast<int32_t*>(lds + 16);
-  float* const s_val = lds + 16 + a.k + 1;
-  const int tid = threadIdx.x;
-  const float lowest = -__builtin_inff();
-  const float inv_t = 1.0f / a.temperature, c_t = kLog2e * inv_t;
-  // without kMix one exponential does for both parts: at T where a = 1, at 1 where a = 0 or T = 1 (c_t is then log2(e) too)
-  const float c = kMix || a.weight > 0.0f ? c_t : kLog2e;
+  const int head = static_cast<int>(std::min<int64_t>(vocab, ((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+  const int vecs = static_cast<int>((vocab - head) / kN);
+  return Body{head, vecs, static_cast<int>(vocab - head - static_cast<int64_t>(vecs) * kN)};
+}
 
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const float up = a.upstream == nullptr ? 1.0f : a.upstream[row * a.upstream_step];
-    if (a.keep_ones && up == 1.0f) continue;
-    const T* const x = static_cast<const T*>(a.logits) + row * a.vocab;
-    T* const g = a.grad == nullptr ? nullptr : static_cast<T*>(a.grad) + row * a.vocab;
-    const int64_t y = a.targets == nullptr ? 0 : index_of(a.targets, a.targets_i64, row);
-    const bool counted = a.targets == nullptr || y != a.ignore;
-    // the row's elements before its first whole vector, and its vectors
-    const int head = static_cast<int>(std::min<int64_t>(a.vocab, ((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int64_t vecs = (a.vocab - head) / kN;
-    const int tail = static_cast<int>(a.vocab - head - vecs * kN);
-    const int64_t edge = tid < head ? tid : tid - head < tail ? head + vecs * kN + (tid - head) : -1;  // this lane's single element
-    if (!counted) {
-      if (a.rows_loss != nullptr && tid == 0) a.rows_loss[row] = 0.0f;
-      if (g != nullptr) {
-        P zero;
-#pragma unroll
-        for (int i = 0; i < kN; ++i) zero.v[i] = narrow<T>(0.0f);
-        for (int64_t v = tid; v < vecs; v += kG) zero.store(g + head + v * kN);
-        if (edge >= 0) g[edge] = narrow<T>(0.0f);
-      }
-      continue;
-    }
+// A running maximum m and the sums of exp2(c (x - m)) (and at log2(e) for the target's share). Where nothing but -inf has been seen the
+// sums are zero and m is -inf; `base` is what stands in for m then. The difference comes first: c x would overflow for masks of the type's
+// lowest value.
+__device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
-    // the teacher
-    const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
-    float bad = hard && (y < 0 || y >= a.vocab) ? 1.0f : 0.0f;
-    float t_max = lowest;
-    __syncthreads();  // the last row's columns and values have been read
-    if (soft)
-      for (int i = tid; i < a.k; i += kG) {
-        const int64_t j = index_of(a.index, a.index_i64, row * a.k + i);
-        float t = teacher_logit(a, row * a.k + i);
-        if (j < 0) t = lowest;
-        if (j >= a.vocab || t != t) bad = 1.0f;
-        s_col[i] = j < 0 || j >= a.vocab ? -1 : static_cast<int32_t>(j);
-        s_val[i] = t;
-        t_max = fmaxf(t_max, t);
-      }
-    t_max = over_row<kG>(t_max, s_red, Max{});
-    bad = over_row<kG>(bad, s_red, Max{});
-    const bool taught = soft && t_max != lowest;  // else no entry says anything
-    float t_sum = 0.0f;
-    if (taught)
-      for (int i = tid; i < a.k; i += kG) {
-        s_val[i] = (s_val[i] - t_max) * inv_t;
-        t_sum += exp2_of(s_val[i] * kLog2e);
-      }
-    t_sum = over_row<kG>(t_sum, s_red, Add{});
+template <bool kMix>
+struct Sums {
+  float m = -__builtin_inff(), z = 0.0f, z1 = 0.0f;
 
-    // the student's maximum and sums, running: z at exponents c (x - m), z1 at log2(e) (x - m)
-    float m = lowest, z = 0.0f, z1 = 0.0f;
-    auto take = [&](float xm, auto each, int n) {  // n elements whose maximum is xm
-      const float top = fmaxf(m, xm);
-      const float base = top == lowest ? 0.0f : top;
-      z *= exp2_of((m - base) * c);
-      if (kMix) z1 *= exp2_of((m - base) * kLog2e);
-      m = top;
+  template <int kN>
+  __device__ __forceinline__ void take(const float (&f)[kN], float c) {
+    float top = f[0];
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        z += exp2_of((each(i) - base) * c);
-        if (kMix) z1 += exp2_of((each(i) - base) * kLog2e);
-      }
-    };
-    for (int64_t v = tid; v < vecs; v += kG) {
-      const P p = P::load(x + head + v * kN);
-      float f[kN], xm = lowest;
+    for (int i = 1; i < kN; ++i) top = fmaxf(top, f[i]);
+    top = fmaxf(top, m);
+    const float base = base_of(top);
+    float s = 0.0f, s1 = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        f[i] = widen(p.v[i]);
-        xm = fmaxf(xm, f[i]);
-      }
-      take(xm, [&](int i) { return f[i]; }, kN);
+    for (int i = 0; i < kN; ++i) {
+      s += exp2_of((f[i] - base) * c);
+      if (kMix) s1 += exp2_of((f[i] - base) * kLog2e);
     }
-    if (edge >= 0) {
-      const float f = widen(x[edge]);
-      take(f, [&](int) { return f; }, 1);
-    }
-    const float top = over_row<kG>(m, s_red, Max{});
-    const float base = top == lowest ? 0.0f : top;
+    z = fmaf(z, exp2_of((m - base) * c), s);
+    if (kMix) z1 = fmaf(z1, exp2_of((m - base) * kLog2e), s1);
+    m = top;
+  }
+  // the same sums with the maximum `top` of several
+  __device__ __forceinline__ void lift(float top, float c) {
+    const float base = base_of(top);
     z *= exp2_of((m - base) * c);
-    z = over_row<kG>(z, s_red, Add{});
-    if (kMix) {
-      z1 *= exp2_of((m - base) * kLog2e);
-      z1 = over_row<kG>(z1, s_red, Add{});
-    } else {
-      z1 = z;
+    if (kMix) z1 *= exp2_of((m - base) * kLog2e);
+    m = top;
+  }
+};
+
+// What a wave knows about a row, for the workgroup's others.
+struct WaveRow {
+  float m, z, z1, t_m, t_z, flags;  // flags: 1 a column named twice, 2 something outside the vocabulary or a NaN of the teacher's
+};
+
+constexpr uint32_t kNoColumn = 0xffffffffu;
+
+// A workgroup of kG lanes per row, and on to the row a grid further. The row is read once into kHeld vectors of every lane's
+// registers (kHeld 0: a row that does not fit is read again for its gradient); every lane keeps its own running maximum and sum, so the
+// exponentials are taken as the vectors arrive, and one barrier joins the waves. While the gradient of a row is computed, each of
+// its vectors makes room for the next row's: loads, exponentials and stores are under way at the same time with one workgroup per
+// compute unit. The teacher's entries are one lane's each (k <= kG): their elements and the target's are written again after the row, behind
+// a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries.
+// kMix: both temperatures are needed (0 < a < 1 and T != 1); otherwise one exponential does for both parts.
+template <typename T, int kG, int kHeld, bool kMix>
+__global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_table) {
+  constexpr int kN = per_vec<T>(), kWaves = kG / kWave;
+  __shared__ WaveRow s_wave[2][kWaves];
+  __shared__ float s_part[2][kWaves];
+  __shared__ int64_t s_cover[2];
+  extern __shared__ uint32_t s_table[];  // 2^log_table columns, then k columns and k values of a row with a column named twice
+  uint32_t* const s_col = s_table + (1 << log_table);
+  float* const s_val = reinterpret_cast<float*>(s_col + a.k);
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
+  const float inv_t = 1.0f / a.temperature;
+  const float c = soft ? kLog2e * inv_t : kLog2e;  // without kMix: T where a = 1, else T = 1 or a = 0
+
+  auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
+
+  Vec16 held[kHeld > 0 ? kHeld : 1];
+  T edge_held = narrow<T>(0.0f);
+  uint32_t col = kNoColumn;  // of the teacher's entry of this lane
+  float t = 0.0f;
+  bool bad = false;
+  const int lane16 = tid * 16;
+  auto body_stretch = [&](const T* x, const Body& b) { return stretch(x + b.head, b.vecs * 16); };
+  auto edge_of = [&](const Body& b) { return tid < b.head ? tid : tid - b.head < b.tail ? b.head + b.vecs * kN + tid - b.head : -1; };
+  auto fetch_small = [&](int64_t row, const T* x, const Body& b) {  // the edge, the teacher's entry
+    const int e = edge_of(b);
+    if (e >= 0) edge_held = x[e];
+    col = kNoColumn;
+    bad = false;
+    t = -__builtin_inff();
+    if (soft && tid < a.k) {
+      const int64_t j = index_of(a.index, a.index_i64, row * a.k + tid);
+      const float logit = teacher_logit(a, row * a.k + tid);
+      if (j >= 0) {
+        bad = j >= a.vocab || logit != logit;
+        if (!bad) {
+          col = static_cast<uint32_t>(j);
+          t = logit;
+        }
+      }
     }
-    const float wrong = bad != 0.0f ? __builtin_nanf("") : 0.0f;  // a column outside the vocabulary shows
+  };
+
+  auto write_zeros = [&](T* g) {
+    const Body b = body_of(g, a.vocab);
+    const Vec16 zero = {0u, 0u, 0u, 0u};
+    for (int v = tid; v < b.vecs; v += kG) __builtin_nontemporal_store(zero, reinterpret_cast<Vec16*>(g + b.head) + v);
+    const int e = edge_of(b);
+    if (e >= 0) g[e] = narrow<T>(0.0f);
+  };
+  // The first row from `row` on, a grid apart, that there is work for; the rows before it that do not count get their zeros. a.rows: none.
+  auto seek = [&](int64_t row) {
+    for (; row < a.rows; row += gridDim.x) {
+      if (a.keep_ones && a.upstream[row * a.upstream_step] == 1.0f) continue;
+      if (a.targets == nullptr || index_of(a.targets, a.targets_i64, row) != a.ignore) return row;
+      if (a.rows_loss != nullptr && tid == 0) a.rows_loss[row] = 0.0f;
+      if (a.grad != nullptr) write_zeros(static_cast<T*>(a.grad) + row * a.vocab);
+    }
+    return a.rows;
+  };
+
+  for (int i = tid; i < 1 << log_table; i += kG) s_table[i] = kNoColumn;
+  if (tid < 2) s_cover[tid] = -1;
+  int64_t row = seek(blockIdx.x);
+  if (row == a.rows) return;
+  Body body = body_of(row_at(row), a.vocab);
+  fetch_small(row, row_at(row), body);
+  if constexpr (kHeld > 0) {
+    const __amdgpu_buffer_rsrc_t from = body_stretch(row_at(row), body);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = load16<kStream>(from, lane16, i * kG * 16);
+  }
+  __syncthreads();
+
+  for (int turn = 0; row < a.rows; turn ^= 1) {
+    const T* const x = row_at(row);
+    T* const g = a.grad == nullptr ? nullptr : static_cast<T*>(a.grad) + row * a.vocab;
+    const float up = a.upstream == nullptr ? 1.0f : a.upstream[row * a.upstream_step];
+    const int64_t y = hard ? index_of(a.targets, a.targets_i64, row) : -1;
+    const bool y_bad = hard && (y < 0 || y >= a.vocab);
+    const int edge = edge_of(body);
+    const float x_col = col != kNoColumn ? widen(x[col]) : 0.0f;
+    const float x_y = hard && !y_bad ? widen(x[y]) : 0.0f;
+    const float edge_x = edge >= 0 ? widen(edge_held) : -__builtin_inff();
+
+    // the row's maximum and sums
+    Sums<kMix> sums;
+    if constexpr (kHeld > 0) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (tid + i * kG < body.vecs) {
+          float f[kN];
+          unpack16<T>(held[i], f);
+          sums.take(f, c);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      for (int v = tid; v < body.vecs; v += kG) {
+        float f[kN];
+        unpack16<T>(reinterpret_cast<const Vec16*>(x + body.head)[v], f);
+        sums.take(f, c);
+      }
+    }
+    {
+      const float f[1] = {edge_x};
+      sums.take(f, c);
+    }
+    // the teacher's, and whether a column comes twice
+    bool twice = false;
+    uint32_t slot = kNoColumn;
+    if (col != kNoColumn) {
+      uint32_t at = (col * 2654435761u) >> (32 - log_table);
+      for (;;) {
+        const uint32_t old = atomicCAS(&s_table[at], kNoColumn, col);
+        if (old == kNoColumn) {
+          slot = at;
+          break;
+        }
+        if (old == col) {
+          twice = true;
+          break;
+        }
+        at = (at + 1) & ((1u << log_table) - 1);
+      }
+    }
+    const float ck = kLog2e * inv_t;
+    WaveRow mine;
+    mine.m = wave_max(sums.m);
+    sums.lift(mine.m, c);
+    mine.z = wave_sum(sums.z);
+    mine.z1 = kMix ? wave_sum(sums.z1) : mine.z;
+    mine.t_m = wave_max(t);
+    mine.t_z = wave_sum(exp2_of((t - base_of(mine.t_m)) * ck));
+    mine.flags = (__ballot(twice) != 0 ? 1.0f : 0.0f) + (__ballot(bad) != 0 ? 2.0f : 0.0f);
+    float m = mine.m, z = mine.z, z1 = mine.z1, t_m = mine.t_m, t_z = mine.t_z;
+    bool any_twice = mine.flags == 1.0f || mine.flags == 3.0f, any_bad = mine.flags >= 2.0f;
+    if constexpr (kWaves > 1) {
+      if (lane == 0) s_wave[turn][wave] = mine;
+      __syncthreads();
+      const bool there = lane < kWaves;
+      WaveRow w = s_wave[turn][there ? lane : 0];
+      if (!there) w.m = w.t_m = -__builtin_inff();
+      if (!there) w.z = w.z1 = w.t_z = w.flags = 0.0f;
+      m = wave_max(w.m);
+      t_m = wave_max(w.t_m);
+      Sums<kMix> part;
+      part.m = w.m;
+      part.z = w.z;
+      part.z1 = w.z1;
+      part.lift(m, c);
+      z = wave_sum(part.z);
+      z1 = kMix ? wave_sum(part.z1) : z;
+      t_z = wave_sum(w.t_z * exp2_of((w.t_m - base_of(t_m)) * ck));
+      any_twice = __ballot(w.flags == 1.0f || w.flags == 3.0f) != 0;
+      any_bad = __ballot(w.flags >= 2.0f) != 0;
+    }
+    any_bad = any_bad || y_bad;
+    const bool taught = soft && t_m != -__builtin_inff();
+    const bool idle = !taught && !hard && !any_bad;  // the teacher says nothing: zeros, whatever the logits are
+    // nothing but -inf: the definition has no value
+    const float wrong = any_bad || (m == -__builtin_inff() && !idle) ? __builtin_nanf("") : 0.0f;
+    const float base = base_of(m);
 
     // the loss
-    const float t2 = a.temperature * a.temperature;
-    float part = 0.0f;
-    const float log_z = ln_of(z), log_t = ln_of(t_sum), p_scale = 1.0f / t_sum;
-    if (taught)
-      for (int i = tid; i < a.k; i += kG) {
-        const float t = s_val[i], p = exp2_of(t * kLog2e) * p_scale;
-        const int j = s_col[i];
-        if (!(p == 0.0f) && j >= 0) part += p * (t - log_t - (widen(x[j]) - top) * inv_t + log_z);
-        s_val[i] = j >= 0 ? p : 0.0f;
-      }
-    part *= a.weight * t2;
-    if (hard && tid == 0 && bad == 0.0f) part += (1.0f - a.weight) * (ln_of(z1) - (widen(x[y]) - top));
-    if (a.rows_loss != nullptr) {
-      part = over_row<kG>(part, s_red, Add{});
-      if (tid == 0) a.rows_loss[row] = part + wrong;
+    float p = 0.0f, part = 0.0f;
+    if (taught && col != kNoColumn) {
+      const float tk = (t - t_m) * inv_t;
+      p = exp2_of(tk * kLog2e) / t_z;
+      if (!(p == 0.0f)) part = a.weight * a.temperature * a.temperature * p * (tk - ln_of(t_z) - ((x_col - base) * inv_t - ln_of(z)));
     }
-    if (g == nullptr) continue;
+    if (hard && tid == 0) part += (1.0f - a.weight) * (ln_of(z1) - (x_y - base));
+    part = wave_sum(part);
+    if (lane == 0) s_part[turn][wave] = part;
 
-    // the gradient: every element from the sums, then the teacher's columns and the target again, with what they take off
+    // the gradient: from the sums, then the teacher's columns and the target again, with what they take off
     const float s = a.scale * up / (a.count == nullptr ? a.divisor : *a.count) + wrong;
     const float w_t = taught ? s * a.weight * a.temperature : 0.0f, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
     const float k_t = (kMix ? w_t : w_t + w_1) / z, k_1 = w_1 / z1;
     auto slope = [&](float f) {
-      float e = k_t * exp2_of((f - top) * c);
-      if (kMix) e += k_1 * exp2_of((f - top) * kLog2e);
+      float e = k_t * exp2_of((f - base) * c);
+      if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
       return e;
     };
-    for (int64_t v = tid; v < vecs; v += kG) {
-      P p = P::load(x + head + v * kN);
-#pragma unroll
-      for (int i = 0; i < kN; ++i) p.v[i] = narrow<T>(slope(widen(p.v[i])));
-      p.store(g + head + v * kN);
+    if (slot != kNoColumn) s_table[slot] = kNoColumn;
+    if (any_twice && tid < a.k) {
+      s_col[tid] = col;
+      s_val[tid] = p;
     }
-    if (edge >= 0) g[edge] = narrow<T>(slope(widen(x[edge])));
-    if (tid == 0) {
-      s_col[a.k] = hard && bad == 0.0f ? static_cast<int32_t>(y) : -1;
-      s_val[a.k] = hard ? w_1 : 0.0f;
+    if (taught && hard && col != kNoColumn && col == static_cast<uint32_t>(y)) s_cover[turn] = row;
+    if (g != nullptr && edge >= 0) g[edge] = narrow<T>(idle ? 0.0f : slope(edge_x) + wrong);
+    if (g != nullptr && idle) write_zeros(g);
+    const uint32_t my_col = col;
+    const int64_t next = seek(row + gridDim.x);
+    const T* const nx = row_at(next < a.rows ? next : row);
+    const Body next_body = body_of(nx, a.vocab);
+    if (next < a.rows) fetch_small(next, nx, next_body);
+    if constexpr (kHeld > 0) {
+      const __amdgpu_buffer_rsrc_t from = stretch(nx + next_body.head, next < a.rows ? next_body.vecs * 16 : 0);
+      const __amdgpu_buffer_rsrc_t to = stretch(g + body.head, g != nullptr && !idle ? body.vecs * 16 : 0);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        if (g != nullptr) {
+          asm("" : "+v"(held[i]));  // unpacked anew: the floats of the sums, kept, would take twice the registers
+          float f[kN];
+          unpack16<T>(held[i], f);
+#pragma unroll
+          for (int e = 0; e < kN; ++e) f[e] = slope(f[e]);
+          store16<kPlain>(pack16<T>(f), to, lane16, i * kG * 16);
+        }
+        held[i] = load16<kStream>(from, lane16, i * kG * 16);
+        __builtin_amdgcn_sched_barrier(0);  // one vector at a time: interleaved, they take twice the registers
+      }
+    } else if (g != nullptr && !idle) {
+      for (int v = tid; v < body.vecs; v += kG) {
+        float f[kN];
+        unpack16<T>(reinterpret_cast<const Vec16*>(x + body.head)[v], f);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) f[e] = slope(f[e]);
+        reinterpret_cast<Vec16*>(g + body.head)[v] = pack16<T>(f);
+      }
     }
     __syncthreads();
-    if (bad == 0.0f)
-      for (int i = tid; i <= a.k; i += kG) {
-        const int j = i == a.k ? s_col[a.k] : taught ? s_col[i] : -1;
-        if (j < 0) continue;
-        float off = 0.0f;  // all that falls on this column: an entry named twice, or the target's, comes out the same for each
-        if (taught)
-          for (int e = 0; e < a.k; ++e) off += s_col[e] == j ? w_t * s_val[e] : 0.0f;
-        if (s_col[a.k] == j) off += s_val[a.k];
-        g[j] = narrow<T>(slope(widen(x[j])) - off);
+    if (a.rows_loss != nullptr && tid == 0) {
+      float loss = wrong;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) loss += s_part[turn][w];
+      a.rows_loss[row] = loss;
+    }
+    if (g != nullptr && !any_bad) {
+      if (taught && my_col != kNoColumn) {
+        float down = w_t * p;  // all that falls on this column: an entry named twice comes out the same for each
+        if (any_twice) {
+          down = 0.0f;
+          for (int e = 0; e < a.k; ++e) down += s_col[e] == my_col ? w_t * s_val[e] : 0.0f;
+        }
+        if (hard && my_col == static_cast<uint32_t>(y)) down += w_1;
+        g[my_col] = narrow<T>(slope(x_col) - down);
       }
+      if (hard && tid == 0 && s_cover[turn] != row) g[y] = narrow<T>(slope(x_y) - w_1);
+    }
+    row = next;
+    body = next_body;
   }
 }
 
 constexpr int kFoldThreads = 1024;
 
-__device__ __forceinline__ float block_sum(float x, float* s) {
-  return over_row<kFoldThreads>(x, s, Add{});
+__device__ __forceinline__ float block_sum(float x) {
+  __shared__ float s[kFoldThreads / kWave];
+  x = wave_sum(x);
+  if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = x;
+  __syncthreads();
+  return wave_sum(threadIdx.x % kWave < kFoldThreads / kWave ? s[threadIdx.x % kWave] : 0.0f);
 }
 
 // How many rows count (at least one: a batch without any has loss 0).
 __global__ __launch_bounds__(kFoldThreads) void distill_count_kernel(const void* targets, int i64, int64_t rows, int64_t ignore, float* count) {
-  __shared__ float s[kFoldThreads / kWave];
   float n = 0.0f;
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < rows; r += kFoldThreads) n += index_of(targets, i64, r) != ignore ? 1.0f : 0.0f;
-  n = block_sum(n, s);
+  n = block_sum(n);
   if (threadIdx.x == 0) *count = fmaxf(n, 1.0f);
 }
 
 __global__ __launch_bounds__(kFoldThreads) void distill_sum_kernel(const float* rows_loss, int64_t rows, const float* count, float divisor, float* loss) {
-  __shared__ float s[kFoldThreads / kWave];
   float x = 0.0f;
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < rows; r += kFoldThreads) x += rows_loss[r];
-  x = block_sum(x, s);
+  x = block_sum(x);
   if (threadIdx.x == 0) *loss = x / (count == nullptr ? divisor : *count);
 }
 
@@ -270,6 +404,7 @@ void check_how(const tdm_distill_how* h) {
 }
 
 constexpr int64_t kCountBytes = 256;
+constexpr int kComputeUnits = 256;
 
 int64_t workspace_bytes_of(const tdm_distill_how& h) { return kCountBytes + (h.reduction == TDM_DISTILL_NONE ? 0 : h.rows * 4); }
 
@@ -336,17 +471,31 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
     a.scale = h.scale;
     if (h.rows > 0) {
       const bool mix = h.weight > 0.0f && h.weight < 1.0f && h.temperature != 1.0f;
-      const unsigned lds = (16 + 2 * (h.k + 1)) * 4;
+      int log_table = 6;  // at most half full
+      while ((1 << log_table) < 2 * h.k) ++log_table;
+      const unsigned lds = ((1u << log_table) + 2u * h.k) * 4u;
       with_dtype(h.dtype, [&](auto t) {
         using T = decltype(t);
         const int64_t vecs = h.vocab * static_cast<int64_t>(sizeof(T)) / 16;
-        auto launch = [&](auto g, auto m) {
-          hipLaunchKernelGGL((distill_kernel<T, g.value, m.value>), dim3(static_cast<unsigned>(std::min<int64_t>(h.rows, 1 << 20))), dim3(g.value), lds, st, a);
+        auto launch = [&](auto g, auto held, auto m) {
+          // as many workgroups as the GPU holds at once: they go on to further rows
+          const int64_t grid = std::min<int64_t>(h.rows, kComputeUnits * (held.value == 0 ? 2 : g.value == 64 ? 32 : 1024 / g.value));
+          hipLaunchKernelGGL((distill_kernel<T, g.value, held.value, m.value>), dim3(static_cast<unsigned>(grid)), dim3(g.value), lds, st, a, log_table);
         };
         auto pick = [&](auto m) {
-          if (vecs <= 128) launch(std::integral_constant<int, 64>{}, m);
-          else if (vecs <= 2048) launch(std::integral_constant<int, 256>{}, m);
-          else launch(std::integral_constant<int, 1024>{}, m);
+          using std::integral_constant;
+          const integral_constant<int, 64> g64{};
+          const integral_constant<int, 256> g256{};
+          const integral_constant<int, 512> g512{};
+          const integral_constant<int, 1024> g1024{};
+          if (h.k <= 64 && vecs <= 64) launch(g64, integral_constant<int, 1>{}, m);
+          else if (h.k <= 64 && vecs <= 256) launch(g64, integral_constant<int, 4>{}, m);
+          else if (h.k <= 256 && vecs <= 1024) launch(g256, integral_constant<int, 4>{}, m);
+          else if (h.k <= 256 && vecs <= 2048) launch(g256, integral_constant<int, 8>{}, m);
+          else if (h.k <= 256 && vecs <= 4096) launch(g256, integral_constant<int, 16>{}, m);
+          else if (h.k <= 512 && vecs <= 8192) launch(g512, integral_constant<int, 16>{}, m);
+          else if (vecs <= 16384) launch(g1024, integral_constant<int, 16>{}, m);
+          else launch(g1024, integral_constant<int, 0>{}, m);
         };
         if (mix) pick(std::true_type{});
         else pick(std::false_type{});

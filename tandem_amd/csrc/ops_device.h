@@ -48,6 +48,82 @@ struct Pack {
   __device__ __forceinline__ void store_nt(T* at) const { __builtin_nontemporal_store(raw(), reinterpret_cast<raw_t*>(at)); }
 };
 
+// 16 bytes of elements that stay packed in four registers (element by element, 16-bit values take a register each).
+typedef uint32_t Vec16 __attribute__((ext_vector_type(4)));
+template <typename T>
+constexpr int per_vec() { return 16 / static_cast<int>(sizeof(T)); }
+template <typename T>
+__device__ __forceinline__ void unpack16(const Vec16& raw, float (&f)[per_vec<T>()]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(raw[i]);
+  } else {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    typedef float pair32 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t word = raw[i];  // a copy: this compiler casts the vector's first element when given raw[i] itself
+      const pair32 x = __builtin_convertvector(__builtin_bit_cast(pair, word), pair32);
+      f[2 * i] = x[0];
+      f[2 * i + 1] = x[1];
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ Vec16 pack16(const float (&f)[per_vec<T>()]) {
+  Vec16 raw;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = __float_as_uint(f[i]);
+  } else {
+    typedef T pair __attribute__((ext_vector_type(2)));
+    typedef float pair32 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair32{f[2 * i], f[2 * i + 1]}, pair));
+  }
+  return raw;
+}
+
+// A stretch of memory for buffer accesses: one register of offsets for many accesses (the rest of an address is scalar), loads
+// behind its end give zeros and stores there do nothing.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t stretch(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);  // raw, 32-bit elements
+}
+constexpr int kPlain = 0, kStream = 2;  // cache policies: cached; non-temporal
+template <int kPolicy>
+__device__ __forceinline__ Vec16 load16(__amdgpu_buffer_rsrc_t from, int lane_offset, int offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, kPolicy);
+}
+template <int kPolicy>
+__device__ __forceinline__ void store16(const Vec16& v, __amdgpu_buffer_rsrc_t to, int lane_offset, int offset) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, to, lane_offset, offset, kPolicy);
+}
+
+// Reductions over the 64 lanes of a wave by DPP: sums along the rows of 16 lanes, then rows 0 and 2 into 1 and 3, then the lower
+// half into the upper; lane 63 has the total, which every lane gets through a scalar register.
+template <int kCtrl, int kRows, class F>
+__device__ __forceinline__ float dpp_step(float x, float none, F f) {
+  return f(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(x), kCtrl, kRows, 0xf, false)));
+}
+struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+template <class F>
+__device__ __forceinline__ float over_16(float x, float none, F f) {  // lane 15 of every row of 16
+  x = dpp_step<0x111, 0xf>(x, none, f);
+  x = dpp_step<0x112, 0xf>(x, none, f);
+  x = dpp_step<0x114, 0xf>(x, none, f);
+  return dpp_step<0x118, 0xf>(x, none, f);
+}
+template <class F>
+__device__ __forceinline__ float over_wave(float x, float none, F f) {
+  x = over_16(x, none, f);
+  x = dpp_step<0x142, 0xa>(x, none, f);
+  x = dpp_step<0x143, 0xc>(x, none, f);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ float wave_sum(float x) { return over_wave(x, 0.0f, Add{}); }
+__device__ __forceinline__ float wave_max(float x) { return over_wave(x, -__builtin_inff(), Max{}); }
+
 // ---- host side
 
 // The widest access, in bytes (16 at most, `least` at least), that divides every one of the addresses and pitches or-ed into `bits`.

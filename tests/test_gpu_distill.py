@@ -201,6 +201,16 @@ def test_what_lies_outside_the_vocabulary_shows_and_stays_in_its_row(vocab):
         assert torch.isnan(grad[wrong]).all() and torch.isfinite(grad[~wrong]).all()
 
 
+def test_a_row_that_the_teacher_says_nothing_about_is_zero_whatever_its_logits():
+    from tandem_amd import ops
+
+    for vocab in (200, 9001, 140000):
+        x, idx, t, y = make(4, vocab, 5, "fp32", 15)
+        x[1, 3], x[2, :], t[1:3] = float("nan"), -INF, -INF
+        loss, grad = ops.distill_loss_and_grad(x, idx, t, reduction="none")
+        assert (loss[1:3] == 0).all() and (grad[1:3] == 0).all() and (loss[[0, 3]] > 0).all()
+
+
 def test_rows_that_start_anywhere():
     from tandem_amd import ops
 
