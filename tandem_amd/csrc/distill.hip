@@ -102,8 +102,29 @@ struct Sums {
 
 // What a wave knows about a row, for the workgroup's others.
 struct WaveRow {
-  float m, z, z1, t_m, t_z, flags;  // flags: 1 a column named twice, 2 something outside the vocabulary or a NaN of the teacher's
+  float m, z, z1, t_m, t_z;
+  uint32_t flags;
 };
+constexpr uint32_t kTwice = 1, kBad = 2;  // a column named twice; something outside the vocabulary, or a NaN of the teacher's
+
+// Over the first kWaves (a power of two, at most 16) lanes of a wave; every lane gets it.
+template <int kWaves>
+__device__ __forceinline__ float sum_of(float x) {
+  if constexpr (kWaves >= 2) x = dpp_step<0x111, 0xf>(x, 0.0f, Add{});
+  if constexpr (kWaves >= 4) x = dpp_step<0x112, 0xf>(x, 0.0f, Add{});
+  if constexpr (kWaves >= 8) x = dpp_step<0x114, 0xf>(x, 0.0f, Add{});
+  if constexpr (kWaves >= 16) x = dpp_step<0x118, 0xf>(x, 0.0f, Add{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWaves - 1));
+}
+template <int kWaves>
+__device__ __forceinline__ float max_of(float x) {
+  const float none = -__builtin_inff();
+  if constexpr (kWaves >= 2) x = dpp_step<0x111, 0xf>(x, none, Max{});
+  if constexpr (kWaves >= 4) x = dpp_step<0x112, 0xf>(x, none, Max{});
+  if constexpr (kWaves >= 8) x = dpp_step<0x114, 0xf>(x, none, Max{});
+  if constexpr (kWaves >= 16) x = dpp_step<0x118, 0xf>(x, none, Max{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), kWaves - 1));
+}
 
 constexpr uint32_t kNoColumn = 0xffffffffu;
 
@@ -130,13 +151,14 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
 
   auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
 
+  constexpr int kEarly = kG >= 1024 ? kHeld / 4 : kHeld;  // vectors of the next row that are read while this row's gradient is written
   Vec16 held[kHeld > 0 ? kHeld : 1];
+  __amdgpu_buffer_rsrc_t from = stretch(nullptr, 0);
   T edge_held = narrow<T>(0.0f);
   uint32_t col = kNoColumn;  // of the teacher's entry of this lane
   float t = 0.0f;
   bool bad = false;
   const int lane16 = tid * 16;
-  auto body_stretch = [&](const T* x, const Body& b) { return stretch(x + b.head, b.vecs * 16); };
   auto edge_of = [&](const Body& b) { return tid < b.head ? tid : tid - b.head < b.tail ? b.head + b.vecs * kN + tid - b.head : -1; };
   auto fetch_small = [&](int64_t row, const T* x, const Body& b) {  // the edge, the teacher's entry
     const int e = edge_of(b);
@@ -182,7 +204,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
   Body body = body_of(row_at(row), a.vocab);
   fetch_small(row, row_at(row), body);
   if constexpr (kHeld > 0) {
-    const __amdgpu_buffer_rsrc_t from = body_stretch(row_at(row), body);
+    from = stretch(row_at(row) + body.head, body.vecs * 16);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) held[i] = load16<kStream>(from, lane16, i * kG * 16);
   }
@@ -223,53 +245,58 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
       sums.take(f, c);
     }
     // the teacher's, and whether a column comes twice
-    bool twice = false;
-    uint32_t slot = kNoColumn;
-    if (col != kNoColumn) {
-      uint32_t at = (col * 2654435761u) >> (32 - log_table);
-      for (;;) {
-        const uint32_t old = atomicCAS(&s_table[at], kNoColumn, col);
-        if (old == kNoColumn) {
-          slot = at;
-          break;
-        }
-        if (old == col) {
-          twice = true;
-          break;
-        }
-        at = (at + 1) & ((1u << log_table) - 1);
-      }
-    }
     const float ck = kLog2e * inv_t;
+    const bool teaches = soft && wave * kWave < a.k;  // this wave has entries
+    uint32_t slot = kNoColumn;
     WaveRow mine;
+    mine.t_m = -__builtin_inff();
+    mine.t_z = 0.0f;
+    mine.flags = 0;
+    if (teaches) {
+      bool twice = false;
+      if (col != kNoColumn) {
+        uint32_t at = (col * 2654435761u) >> (32 - log_table);
+        for (;;) {
+          const uint32_t old = atomicCAS(&s_table[at], kNoColumn, col);
+          if (old == kNoColumn) {
+            slot = at;
+            break;
+          }
+          if (old == col) {
+            twice = true;
+            break;
+          }
+          at = (at + 1) & ((1u << log_table) - 1);
+        }
+      }
+      mine.t_m = wave_max(t);
+      mine.t_z = wave_sum(exp2_of((t - base_of(mine.t_m)) * ck));
+      mine.flags = (__ballot(twice) != 0 ? kTwice : 0) | (__ballot(bad) != 0 ? kBad : 0);
+    }
     mine.m = wave_max(sums.m);
     sums.lift(mine.m, c);
     mine.z = wave_sum(sums.z);
     mine.z1 = kMix ? wave_sum(sums.z1) : mine.z;
-    mine.t_m = wave_max(t);
-    mine.t_z = wave_sum(exp2_of((t - base_of(mine.t_m)) * ck));
-    mine.flags = (__ballot(twice) != 0 ? 1.0f : 0.0f) + (__ballot(bad) != 0 ? 2.0f : 0.0f);
     float m = mine.m, z = mine.z, z1 = mine.z1, t_m = mine.t_m, t_z = mine.t_z;
-    bool any_twice = mine.flags == 1.0f || mine.flags == 3.0f, any_bad = mine.flags >= 2.0f;
+    bool any_twice = mine.flags & kTwice, any_bad = mine.flags & kBad;
     if constexpr (kWaves > 1) {
       if (lane == 0) s_wave[turn][wave] = mine;
       __syncthreads();
-      const bool there = lane < kWaves;
-      WaveRow w = s_wave[turn][there ? lane : 0];
-      if (!there) w.m = w.t_m = -__builtin_inff();
-      if (!there) w.z = w.z1 = w.t_z = w.flags = 0.0f;
-      m = wave_max(w.m);
-      t_m = wave_max(w.t_m);
+      const WaveRow w = s_wave[turn][lane % kWaves];  // at most 16 waves: every row of 16 lanes has them all, some more than once
+      m = max_of<kWaves>(w.m);
       Sums<kMix> part;
       part.m = w.m;
       part.z = w.z;
       part.z1 = w.z1;
       part.lift(m, c);
-      z = wave_sum(part.z);
-      z1 = kMix ? wave_sum(part.z1) : z;
-      t_z = wave_sum(w.t_z * exp2_of((w.t_m - base_of(t_m)) * ck));
-      any_twice = __ballot(w.flags == 1.0f || w.flags == 3.0f) != 0;
-      any_bad = __ballot(w.flags >= 2.0f) != 0;
+      z = sum_of<kWaves>(part.z);
+      z1 = kMix ? sum_of<kWaves>(part.z1) : z;
+      if (soft) {
+        t_m = max_of<kWaves>(w.t_m);
+        t_z = sum_of<kWaves>(w.t_z * exp2_of((w.t_m - base_of(t_m)) * ck));
+      }
+      any_twice = __ballot(w.flags & kTwice) != 0;
+      any_bad = __ballot(w.flags & kBad) != 0;
     }
     any_bad = any_bad || y_bad;
     const bool taught = soft && t_m != -__builtin_inff();
@@ -279,31 +306,34 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     const float base = base_of(m);
 
     // the loss
-    float p = 0.0f, part = 0.0f;
-    if (taught && col != kNoColumn) {
-      const float tk = (t - t_m) * inv_t;
-      p = exp2_of(tk * kLog2e) / t_z;
-      if (!(p == 0.0f)) part = a.weight * a.temperature * a.temperature * p * (tk - ln_of(t_z) - ((x_col - base) * inv_t - ln_of(z)));
+    float p = 0.0f;
+    if (teaches || wave == 0) {
+      float part = 0.0f;
+      if (taught && col != kNoColumn) {
+        const float tk = (t - t_m) * inv_t;
+        p = exp2_of(tk * kLog2e) / t_z;
+        if (!(p == 0.0f)) part = a.weight * a.temperature * a.temperature * p * (tk - ln_of(t_z) - ((x_col - base) * inv_t - ln_of(z)));
+      }
+      if (hard && tid == 0) part += (1.0f - a.weight) * (ln_of(z1) - (x_y - base));
+      part = wave_sum(part);
+      if (lane == 0) s_part[turn][wave] = part;
+      if (slot != kNoColumn) s_table[slot] = kNoColumn;
+      if (any_twice && tid < a.k) {
+        s_col[tid] = col;
+        s_val[tid] = p;
+      }
+      if (taught && hard && col != kNoColumn && col == static_cast<uint32_t>(y)) s_cover[turn] = row;
     }
-    if (hard && tid == 0) part += (1.0f - a.weight) * (ln_of(z1) - (x_y - base));
-    part = wave_sum(part);
-    if (lane == 0) s_part[turn][wave] = part;
 
     // the gradient: from the sums, then the teacher's columns and the target again, with what they take off
     const float s = a.scale * up / (a.count == nullptr ? a.divisor : *a.count) + wrong;
-    const float w_t = taught ? s * a.weight * a.temperature : 0.0f, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
+    const float w_t = taught ? s * a.weight * a.temperature : wrong, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
     const float k_t = (kMix ? w_t : w_t + w_1) / z, k_1 = w_1 / z1;
     auto slope = [&](float f) {
       float e = k_t * exp2_of((f - base) * c);
       if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
       return e;
     };
-    if (slot != kNoColumn) s_table[slot] = kNoColumn;
-    if (any_twice && tid < a.k) {
-      s_col[tid] = col;
-      s_val[tid] = p;
-    }
-    if (taught && hard && col != kNoColumn && col == static_cast<uint32_t>(y)) s_cover[turn] = row;
     if (g != nullptr && edge >= 0) g[edge] = narrow<T>(idle ? 0.0f : slope(edge_x) + wrong);
     if (g != nullptr && idle) write_zeros(g);
     const uint32_t my_col = col;
@@ -311,9 +341,15 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     const T* const nx = row_at(next < a.rows ? next : row);
     const Body next_body = body_of(nx, a.vocab);
     if (next < a.rows) fetch_small(next, nx, next_body);
+    // 16-bit gradients: one multiply-add and the exponential, k and the row's maximum in the exponent, the sign of k apart. That is off by
+    // 2^-24 of the exponent's terms: far less than the store's rounding while they stay below 1024. Other rows, and
+    // what does not fit the registers, are read again.
+    const float off = log2f(fabsf(k_t)) - base * c, off1 = kMix ? log2f(fabsf(k_1)) - base * kLog2e : 0.0f;
+    const uint32_t sign = s < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+    const bool held_fits = sizeof(T) == 4 || (fabsf(base * c) < 1024.0f && (!kMix || fabsf(base * kLog2e) < 1024.0f));
     if constexpr (kHeld > 0) {
-      const __amdgpu_buffer_rsrc_t from = stretch(nx + next_body.head, next < a.rows ? next_body.vecs * 16 : 0);
-      const __amdgpu_buffer_rsrc_t to = stretch(g + body.head, g != nullptr && !idle ? body.vecs * 16 : 0);
+      from = stretch(nx + next_body.head, next < a.rows ? next_body.vecs * 16 : 0);
+      const __amdgpu_buffer_rsrc_t to = stretch(g + body.head, g != nullptr && !idle && held_fits ? body.vecs * 16 : 0);
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         if (g != nullptr) {
@@ -321,13 +357,19 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
           float f[kN];
           unpack16<T>(held[i], f);
 #pragma unroll
-          for (int e = 0; e < kN; ++e) f[e] = slope(f[e]);
-          store16<kPlain>(pack16<T>(f), to, lane16, i * kG * 16);
+          for (int e = 0; e < kN; ++e) {
+            if constexpr (sizeof(T) == 4) f[e] = slope(f[e]);
+            else f[e] = exp2_of(fmaf(f[e], c, off)) + (kMix ? exp2_of(fmaf(f[e], kLog2e, off1)) : 0.0f);
+          }
+          Vec16 out = pack16<T>(f);
+          if constexpr (sizeof(T) == 2) out ^= sign;
+          store16<kPlain>(out, to, lane16, i * kG * 16);
         }
-        held[i] = load16<kStream>(from, lane16, i * kG * 16);
+        if (i < kEarly) held[i] = load16<kStream>(from, lane16, i * kG * 16);
         __builtin_amdgcn_sched_barrier(0);  // one vector at a time: interleaved, they take twice the registers
       }
-    } else if (g != nullptr && !idle) {
+    }
+    if (g != nullptr && !idle && (kHeld == 0 || !held_fits)) {
       for (int v = tid; v < body.vecs; v += kG) {
         float f[kN];
         unpack16<T>(reinterpret_cast<const Vec16*>(x + body.head)[v], f);
@@ -337,10 +379,15 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
       }
     }
     __syncthreads();
+    if constexpr (kHeld > 0) {
+#pragma unroll
+      for (int i = kEarly; i < kHeld; ++i) held[i] = load16<kStream>(from, lane16, i * kG * 16);
+    }
     if (a.rows_loss != nullptr && tid == 0) {
       float loss = wrong;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) loss += s_part[turn][w];
+      for (int w = 0; w < kWaves; ++w)
+        if (w == 0 || (soft && w * kWave < a.k)) loss += s_part[turn][w];
       a.rows_loss[row] = loss;
     }
     if (g != nullptr && !any_bad) {

@@ -187,6 +187,21 @@ def test_a_teacher_s_column_that_the_student_masks_costs_infinity():
     check(x, idx, t, None, 1.0, 1.0, "none")
 
 
+@pytest.mark.parametrize("dtype,shift", [("bf16", 3000.0), ("bf16", -2.0 ** 100), ("fp16", -60000.0), ("fp32", 1.0e30), ("bf16", 40.0)])
+@pytest.mark.parametrize("vocab", [250, 3001, 40000, 100000])
+def test_rows_far_from_zero(vocab, dtype, shift):
+    """Softmax does not depend on a constant that all logits share: rows of two values of the type, `shift` and the next one up (or,
+    where that is a step of more than 64, infinitely less likely ones), against the reference."""
+    x, idx, t, y = make(6, vocab, 9, dtype, 16)
+    low = torch.full((), shift, dtype=x.dtype, device=DEV)
+    high = torch.nextafter(low.float() if dtype == "fp32" else low, torch.full((), INF, dtype=x.dtype, device=DEV))
+    x = torch.where(x > 0, low, high)
+    if float(high) - float(low) > 64:
+        x = low.expand(6, vocab).contiguous()
+    check(x, idx, t, y, 2.0, 0.5, scale=256.0)
+    check(x, idx, t, None, 1.0, 1.0, scale=-256.0)
+
+
 @pytest.mark.parametrize("vocab", [100, 9001])
 def test_what_lies_outside_the_vocabulary_shows_and_stays_in_its_row(vocab):
     from tandem_amd import ops
