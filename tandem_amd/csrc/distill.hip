@@ -136,7 +136,7 @@ constexpr uint32_t kNoColumn = 0xffffffffu;
 // a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries.
 // kMix: both temperatures are needed (0 < a < 1 and T != 1); otherwise one exponential does for both parts.
 template <typename T, int kG, int kHeld, bool kMix>
-__global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_table) {
+__global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(DistillArgs a, int log_table) {
   constexpr int kN = per_vec<T>(), kWaves = kG / kWave;
   __shared__ WaveRow s_wave[2][kWaves];
   __shared__ float s_part[2][kWaves];
@@ -146,27 +146,30 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
   float* const s_val = reinterpret_cast<float*>(s_col + a.k);
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
-  const float inv_t = 1.0f / a.temperature;
+  const float inv_t = 1.0f / a.temperature, scale = a.scale / (a.count == nullptr ? a.divisor : *a.count);
   const float c = soft ? kLog2e * inv_t : kLog2e;  // without kMix: T where a = 1, else T = 1 or a = 0
 
   auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
 
-  constexpr int kEarly = kG >= 1024 ? kHeld / 4 : kHeld;  // vectors of the next row that are read while this row's gradient is written
+  constexpr int kEarly = kHeld / 2;  // vectors of the next row that are read while this row's gradient is written
   Vec16 held[kHeld > 0 ? kHeld : 1];
   __amdgpu_buffer_rsrc_t from = stretch(nullptr, 0);
   T edge_held = narrow<T>(0.0f);
   uint32_t col = kNoColumn;  // of the teacher's entry of this lane
-  float t = 0.0f;
+  float t = -__builtin_inff();
   bool bad = false;
   const int lane16 = tid * 16;
   auto edge_of = [&](const Body& b) { return tid < b.head ? tid : tid - b.head < b.tail ? b.head + b.vecs * kN + tid - b.head : -1; };
   auto fetch_small = [&](int64_t row, const T* x, const Body& b) {  // the edge, the teacher's entry
-    const int e = edge_of(b);
-    if (e >= 0) edge_held = x[e];
+    if (wave == 0) {
+      const int e = edge_of(b);
+      if (e >= 0) edge_held = x[e];
+    }
+    if (!soft || wave * kWave >= a.k) return;
     col = kNoColumn;
     bad = false;
     t = -__builtin_inff();
-    if (soft && tid < a.k) {
+    if (tid < a.k) {
       const int64_t j = index_of(a.index, a.index_i64, row * a.k + tid);
       const float logit = teacher_logit(a, row * a.k + tid);
       if (j >= 0) {
@@ -220,6 +223,10 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     const float x_col = col != kNoColumn ? widen(x[col]) : 0.0f;
     const float x_y = hard && !y_bad ? widen(x[y]) : 0.0f;
     const float edge_x = edge >= 0 ? widen(edge_held) : -__builtin_inff();
+
+    const int64_t next = seek(row + gridDim.x);
+    const T* const nx = row_at(next < a.rows ? next : row);
+    const Body next_body = body_of(nx, a.vocab);
 
     // the row's maximum and sums
     Sums<kMix> sums;
@@ -326,9 +333,9 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     }
 
     // the gradient: from the sums, then the teacher's columns and the target again, with what they take off
-    const float s = a.scale * up / (a.count == nullptr ? a.divisor : *a.count) + wrong;
+    const float s = scale * up + wrong;
     const float w_t = taught ? s * a.weight * a.temperature : wrong, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
-    const float k_t = (kMix ? w_t : w_t + w_1) / z, k_1 = w_1 / z1;
+    const float k_t = (kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z), k_1 = kMix ? w_1 * __builtin_amdgcn_rcpf(z1) : 0.0f;
     auto slope = [&](float f) {
       float e = k_t * exp2_of((f - base) * c);
       if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
@@ -337,14 +344,11 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     if (g != nullptr && edge >= 0) g[edge] = narrow<T>(idle ? 0.0f : slope(edge_x) + wrong);
     if (g != nullptr && idle) write_zeros(g);
     const uint32_t my_col = col;
-    const int64_t next = seek(row + gridDim.x);
-    const T* const nx = row_at(next < a.rows ? next : row);
-    const Body next_body = body_of(nx, a.vocab);
     if (next < a.rows) fetch_small(next, nx, next_body);
     // 16-bit gradients: one multiply-add and the exponential, k and the row's maximum in the exponent, the sign of k apart. That is off by
     // 2^-24 of the exponent's terms: far less than the store's rounding while they stay below 1024. Other rows, and
     // what does not fit the registers, are read again.
-    const float off = log2f(fabsf(k_t)) - base * c, off1 = kMix ? log2f(fabsf(k_1)) - base * kLog2e : 0.0f;
+    const float off = __builtin_amdgcn_logf(fabsf(k_t)) - base * c, off1 = kMix ? __builtin_amdgcn_logf(fabsf(k_1)) - base * kLog2e : 0.0f;
     const uint32_t sign = s < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
     const bool held_fits = sizeof(T) == 4 || (fabsf(base * c) < 1024.0f && (!kMix || fabsf(base * kLog2e) < 1024.0f));
     if constexpr (kHeld > 0) {
@@ -363,7 +367,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
           }
           Vec16 out = pack16<T>(f);
           if constexpr (sizeof(T) == 2) out ^= sign;
-          store16<kPlain>(out, to, lane16, i * kG * 16);
+          store16<kStream>(out, to, lane16, i * kG * 16);
         }
         if (i < kEarly) held[i] = load16<kStream>(from, lane16, i * kG * 16);
         __builtin_amdgcn_sched_barrier(0);  // one vector at a time: interleaved, they take twice the registers
@@ -526,7 +530,7 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
         const int64_t vecs = h.vocab * static_cast<int64_t>(sizeof(T)) / 16;
         auto launch = [&](auto g, auto held, auto m) {
           // as many workgroups as the GPU holds at once: they go on to further rows
-          const int64_t grid = std::min<int64_t>(h.rows, kComputeUnits * (held.value == 0 ? 2 : g.value == 64 ? 32 : 1024 / g.value));
+          const int64_t grid = std::min<int64_t>(h.rows, kComputeUnits * (held.value == 0 ? 2 : g.value == 64 ? 32 : (held.value > 16 ? 512 : 1024) / g.value));
           hipLaunchKernelGGL((distill_kernel<T, g.value, held.value, m.value>), dim3(static_cast<unsigned>(grid)), dim3(g.value), lds, st, a, log_table);
         };
         auto pick = [&](auto m) {
