@@ -6,6 +6,7 @@ caller gets an exception. Nothing here computes on the CPU.
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -56,27 +57,11 @@ class AdamwHyper(ctypes.Structure):
                 ("eps", ctypes.c_double), ("neg_step", ctypes.c_double)]
 
 
-class HeadsView(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
-
-
-class Positions(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64)]
-
-
-class QkShape(ctypes.Structure):
-    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
-                ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32),
-                ("weight_dtype", ctypes.c_int32), ("position_dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
-
-
-class DistillHow(ctypes.Structure):
-    _fields_ = [("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("ignore_index", ctypes.c_int64), ("k", ctypes.c_int32),
-                ("dtype", ctypes.c_int32), ("index_dtype", ctypes.c_int32), ("teacher_dtype", ctypes.c_int32), ("target_dtype", ctypes.c_int32),
-                ("reduction", ctypes.c_int32), ("temperature", ctypes.c_float), ("weight", ctypes.c_float), ("scale", ctypes.c_float)]
-
-
-_PHEADS, _PSHAPE, _PPOSITIONS = ctypes.POINTER(HeadsView), ctypes.POINTER(QkShape), ctypes.POINTER(Positions)
+# The operators' structures, packed by the caller: a call passes their bytes (tdm_heads, tdm_positions, tdm_qk_shape, tdm_distill_how).
+HEADS = struct.Struct("Qqqq")
+POSITIONS = struct.Struct("Qqq")
+QK_SHAPE = struct.Struct("qq8if4x")
+DISTILL_HOW = struct.Struct("qqq6i3f4x")
 
 _SIGNATURES = {
     "tdm_last_error": (ctypes.c_char_p, []),
@@ -138,14 +123,14 @@ _SIGNATURES = {
     "tdm_k5_embedding_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_int64,
                                              ctypes.c_void_p]),
-    "tdm_k6_qk_norm_rope": (ctypes.c_int, [_PSHAPE, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p, _PPOSITIONS, ctypes.c_void_p,
-                                           _PHEADS, _PHEADS, ctypes.c_void_p]),
-    "tdm_k6_qk_norm_rope_grad_workspace": (ctypes.c_int64, [_PSHAPE]),
-    "tdm_k6_qk_norm_rope_grad": (ctypes.c_int, [_PSHAPE, _PHEADS, _PHEADS, _PHEADS, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p,
-                                                _PPOSITIONS, ctypes.c_void_p, _PHEADS, _PHEADS, _PHEADS, ctypes.c_void_p, ctypes.c_void_p,
+    "tdm_k6_qk_norm_rope": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p,
+                                           ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p]),
+    "tdm_k6_qk_norm_rope_grad_workspace": (ctypes.c_int64, [ctypes.c_char_p]),
+    "tdm_k6_qk_norm_rope_grad": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_char_p, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
-    "tdm_k7_distill_workspace": (ctypes.c_int64, [ctypes.POINTER(DistillHow)]),
-    "tdm_k7_distill": (ctypes.c_int, [ctypes.POINTER(DistillHow), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+    "tdm_k7_distill_workspace": (ctypes.c_int64, [ctypes.c_char_p]),
+    "tdm_k7_distill": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
                                       ctypes.c_void_p]),
 }

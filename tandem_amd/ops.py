@@ -9,44 +9,60 @@ captured into a graph. The reference has no counterpart: its model (tandem/model
 operators.
 """
 
-import ctypes
+import struct
 
 import torch
 
-from ._lib import DistillHow, HeadsView, Positions, QkShape, check, dtype_code, lib, require_device_tensor, stream_ptr
+from ._lib import DISTILL_HOW, DTYPES as CODES, HEADS, POSITIONS, QK_SHAPE, check, lib, require_device_tensor
 
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 INDEX_DTYPES = (torch.int64, torch.int32)
 
 
+def _on_gpu(t, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{what}: needs a tensor in GPU memory (got {getattr(t, 'device', type(t))}); tandem_amd has no CPU path")
+
+
 def _floating(t, what):
-    require_device_tensor(t, what)
+    _on_gpu(t, what)
     if t.dtype not in DTYPES:
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: needs a contiguous tensor")
 
 
 def _indices(t, what):
     """`t` as contiguous indices in GPU memory (slices of a batch are copied)."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
-        raise ValueError(f"{what}: needs a tensor in GPU memory (got {getattr(t, 'device', type(t))}); tandem_amd has no CPU path")
+    _on_gpu(t, what)
     if t.dtype not in INDEX_DTYPES:
         raise ValueError(f"{what}: int64 or int32, not {t.dtype}")
     return t.contiguous()
 
 
 def _same_device(first, *others):
+    device = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != device:
             raise ValueError(f"tensors on {first.device} and {t.device}")
 
 
-def _call(device, entry, *args):
-    """entry(*args, stream) on `device`'s current stream: the launch goes to the current device, which may be another."""
-    if device.index == torch.cuda.current_device():
-        check(entry(*args, stream_ptr(device)))
+def _call(t, entry, *args):
+    """entry(*args, stream) on the current stream of `t`'s device: the launch goes to the current device, which may be another."""
+    device = t.get_device()
+    if device == torch.cuda.current_device():
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            check(entry(*args, stream_ptr(device)))
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        check(status)
+
+
+def _workspace(bytes_needed, like):
+    if bytes_needed < 0:
+        raise ValueError(lib().tdm_last_error().decode(errors="replace"))
+    return torch.empty(bytes_needed, device=like.device, dtype=torch.uint8)
 
 
 # ---- embedding
@@ -85,8 +101,8 @@ def _embedding(tokens, weight, scale):
     _same_device(weight, tokens)
     vocab, dim = weight.shape
     out = torch.empty(*tokens.shape, dim, device=weight.device, dtype=weight.dtype)
-    _call(weight.device, lib().tdm_k5_embedding, weight.data_ptr(), tokens.data_ptr(), dtype_code(tokens.dtype), out.data_ptr(),
-          tokens.numel(), vocab, dim, dtype_code(weight.dtype), scale)
+    _call(weight, lib().tdm_k5_embedding, weight.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), tokens.numel(), vocab, dim,
+          CODES[weight.dtype], scale)
     return out
 
 
@@ -110,11 +126,9 @@ def _embedding_grad(grad, tokens, vocab, scale, padding):
     out = torch.empty(vocab, dim, device=grad.device, dtype=grad.dtype)
     L = lib()
     need = L.tdm_k5_embedding_grad_workspace(n, vocab, dim)
-    if need < 0:
-        raise ValueError(L.tdm_last_error().decode(errors="replace"))
-    work = torch.empty(need, device=grad.device, dtype=torch.uint8)
-    _call(grad.device, L.tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), dtype_code(tokens.dtype), out.data_ptr(),
-          work.data_ptr(), need, n, vocab, dim, dtype_code(grad.dtype), scale, padding)
+    work = _workspace(need, grad)
+    _call(grad, L.tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), work.data_ptr(), need, n, vocab, dim,
+          CODES[grad.dtype], scale, padding)
     return out
 
 
@@ -154,49 +168,105 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
     same dtype or float32. positions: int64 or int32, of a shape that expands to [batch, tokens]; inv_freq: float64
     (rope_frequencies). Angles are computed in float64, so far positions keep their precision. Single tokens are a
     batch of one token each."""
-    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QkNormRope.apply(q, k, q_weight, k_weight, how)
-    return _qk_forward(q, k, q_weight, k_weight, how)
+    x = _separate(q, k)
+    how = _check_qk(x, q, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or _wants_grad(q_weight) or _wants_grad(k_weight)):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, x, how)
+    return _qk_forward(q, q_weight, k_weight, x, how)
 
 
 def qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """The gradients (dq, dk, dq_weight, dk_weight) of qk_norm_rope for the upstream gradients dq_out, dk_out (None: zeros); a
     weight that is None has none. The weights' gradients are summed in fp32 over all tokens and heads in a fixed order."""
-    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    dq, dk = torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype)
-    return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, k, q_weight, k_weight, how, dq, dk, None))
+    x = _separate(q, k)
+    how = _check_qk(x, q, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    return _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how)
 
 
 def qkv_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """qk_norm_rope on a packed projection: qkv [batch, tokens, (q_heads + 2 kv_heads) * dim] (or without batch) holds the
     queries' heads, the keys' and the values'. Returns (q, k, v): q and k as qk_norm_rope does, v a view of qkv. Its gradient
     is one pass that writes the gradient of qkv whole, the values' part included."""
-    q, k, v = _split_qkv(qkv, q_heads, kv_heads)
-    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight)):
-        return _QkvNormRope.apply(qkv, q_heads, kv_heads, q_weight, k_weight, how)
-    return (*_qk_forward(q, k, q_weight, k_weight, how), v)
+    x = _packed(qkv, q_heads, kv_heads)
+    how = _check_qk(x, qkv, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    if torch.is_grad_enabled() and (qkv.requires_grad or _wants_grad(q_weight) or _wants_grad(k_weight)):
+        return _QkvNormRope.apply(qkv, q_weight, k_weight, x, how)
+    return (*_qk_forward(qkv, q_weight, k_weight, x, how), _values(qkv, x))
 
 
 def qkv_norm_rope_grad(dq_out, dk_out, dv_out, qkv, q_heads, kv_heads, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
     """The gradients (dqkv, dq_weight, dk_weight) of qkv_norm_rope for the upstream gradients dq_out, dk_out, dv_out (None: zeros)."""
-    q, k, v = _split_qkv(qkv, q_heads, kv_heads)
-    how = _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
-    return (dqkv, *_qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, how, *_split_qkv(dqkv, q_heads, kv_heads)))
+    x = _packed(qkv, q_heads, kv_heads)
+    how = _check_qk(x, qkv, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    return _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how)
 
 
-def _split_qkv(qkv, q_heads, kv_heads):
-    if not isinstance(qkv, torch.Tensor) or qkv.dim() not in (2, 3):
-        raise ValueError("qkv: [batch, tokens, width] or [tokens, width]")
+class _Heads:
+    """Where a call's heads lie: tokens ((batch, tokens) or (tokens,)), heads and their size, and q, k and, packed, v as tdm_heads."""
+
+    __slots__ = ("tokens", "q_heads", "kv_heads", "dim", "q", "k", "v")
+
+
+def _tensor(t, what):
+    _on_gpu(t, what)
+    if t.dtype not in DTYPES:
+        raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
+
+
+def _packed(qkv, q_heads, kv_heads):
+    _tensor(qkv, "qkv")
+    *tokens, width = qkv.shape
+    if len(tokens) not in (1, 2) or qkv.stride(-1) != 1:
+        raise ValueError(f"qkv {list(qkv.shape)}: [batch, tokens, width] or [tokens, width], the last dimension contiguous")
     heads = q_heads + 2 * kv_heads
-    if q_heads < 1 or kv_heads < 1 or qkv.shape[-1] == 0 or qkv.shape[-1] % heads:
-        raise ValueError(f"qkv: a width of {qkv.shape[-1]} for {q_heads} query heads and {kv_heads} key and value heads")
-    if qkv.stride(-1) != 1:
-        raise ValueError("qkv: the last dimension must be contiguous")
-    x = qkv.unflatten(-1, (heads, -1))
-    return x[..., :q_heads, :], x[..., q_heads:q_heads + kv_heads, :], x[..., q_heads + kv_heads:, :]
+    if q_heads < 1 or kv_heads < 1 or width == 0 or width % heads:
+        raise ValueError(f"qkv: a width of {width} for {q_heads} query heads and {kv_heads} key and value heads")
+    x = _Heads()
+    x.tokens, x.q_heads, x.kv_heads, x.dim = tokens, q_heads, kv_heads, width // heads
+    _place_packed(x, qkv)
+    return x
+
+
+def _place_packed(x, qkv):
+    strides = qkv.stride()
+    lead = strides[:-1] if len(strides) == 3 else (0, strides[0])
+    at, step = qkv.data_ptr(), x.dim * qkv.element_size()
+    x.q = HEADS.pack(at, *lead, x.dim)
+    x.k = HEADS.pack(at + x.q_heads * step, *lead, x.dim)
+    x.v = HEADS.pack(at + (x.q_heads + x.kv_heads) * step, *lead, x.dim)
+
+
+def _values(qkv, x):
+    """The values' heads, a view."""
+    return qkv.as_strided((*x.tokens, x.kv_heads, x.dim), (*qkv.stride()[:-1], x.dim, 1),
+                          qkv.storage_offset() + (x.q_heads + x.kv_heads) * x.dim)
+
+
+def _separate(q, k):
+    _tensor(q, "q")
+    _tensor(k, "k")
+    *tokens, q_heads, dim = q.shape
+    *k_tokens, kv_heads, k_dim = k.shape
+    if q.dtype != k.dtype or tokens != k_tokens or dim != k_dim:
+        raise ValueError(f"q {list(q.shape)} {q.dtype} and k {list(k.shape)} {k.dtype} differ in dtype, tokens or head size")
+    if len(tokens) not in (1, 2) or 0 in (q_heads, kv_heads, dim) or q.stride(-1) != 1 or k.stride(-1) != 1:
+        raise ValueError(f"q {list(q.shape)}, k {list(k.shape)}: [batch, tokens, heads, dim] or [tokens, heads, dim], the last dimension contiguous")
+    _same_device(q, k)
+    x = _Heads()
+    x.tokens, x.q_heads, x.kv_heads, x.dim, x.q, x.k, x.v = tokens, q_heads, kv_heads, dim, _view(q), _view(k), None
+    return x
+
+
+def _view(t):
+    """t [batch, tokens, heads, dim] or [tokens, heads, dim] as tdm_heads; None: no data."""
+    if t is None:
+        return HEADS.pack(0, 0, 0, 0)
+    strides = t.stride()
+    return HEADS.pack(t.data_ptr(), *strides[:-1]) if len(strides) == 4 else HEADS.pack(t.data_ptr(), 0, *strides[:-1])
+
+
+def _wants_grad(w):
+    return w is not None and w.requires_grad
 
 
 class _QkHow:
@@ -205,124 +275,117 @@ class _QkHow:
     __slots__ = ("shape", "positions", "at", "inv_freq")
 
 
-def _check_qk(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved):
-    for t, what in ((q, "q"), (k, "k")):
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
-            raise ValueError(f"qk_norm_rope({what}): needs a tensor in GPU memory (got {getattr(t, 'device', type(t))}); tandem_amd has no CPU path")
-        if t.dtype not in DTYPES:
-            raise ValueError(f"qk_norm_rope({what}): float32, float16 or bfloat16, not {t.dtype}")
-        if t.dim() not in (3, 4) or 0 in t.shape[-2:] or t.stride(-1) != 1:
-            raise ValueError(f"qk_norm_rope({what}): [batch, tokens, heads, dim] or [tokens, heads, dim], the last dimension contiguous")
-    if q.dtype != k.dtype or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
-        raise ValueError(f"q {list(q.shape)} {q.dtype} and k {list(k.shape)} {k.dtype} differ in dtype, tokens or head size")
-    dim = q.shape[-1]
-    weight_dtype = q.dtype
+def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved):
+    dtype = weight_dtype = like.dtype
     for w in (q_weight, k_weight):
-        if w is None:
-            continue
-        _floating(w, "qk_norm_rope(weight)")
-        if w.shape != (dim,) or w.dtype not in (q.dtype, torch.float32):
-            raise ValueError(f"a weight of {list(w.shape)} {w.dtype} for heads of {dim} {q.dtype}")
-        weight_dtype = w.dtype
+        if w is not None:
+            _floating(w, "qk_norm_rope(weight)")
+            weight_dtype = w.dtype
+            if w.shape != (x.dim,) or weight_dtype not in (dtype, torch.float32):
+                raise ValueError(f"a weight of {list(w.shape)} {w.dtype} for heads of {x.dim} {dtype}")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError("q_weight and k_weight differ in dtype")
     if not isinstance(positions, torch.Tensor) or positions.dtype not in INDEX_DTYPES:
         raise ValueError("positions: an int64 or int32 tensor")
     require_device_tensor(inv_freq, "qk_norm_rope(inv_freq)")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > dim:
-        raise ValueError(f"inv_freq: at most {dim // 2} float64 values")
-    _same_device(q, k, q_weight, k_weight, positions, inv_freq)
-    tokens = q.shape[:-2]
-    how = _QkHow()
-    if positions.shape != tokens:
+    rotary = 2 * inv_freq.numel()
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or rotary > x.dim:
+        raise ValueError(f"inv_freq: at most {x.dim // 2} float64 values")
+    _same_device(like, q_weight, k_weight, positions, inv_freq)
+    tokens = x.tokens
+    if list(positions.shape) != tokens:
         try:
             positions = positions.expand(tokens)
         except RuntimeError:
-            raise ValueError(f"positions of {list(positions.shape)} for tokens of {list(tokens)}") from None
+            raise ValueError(f"positions of {list(positions.shape)} for tokens of {tokens}") from None
+    how = _QkHow()
     how.positions, how.inv_freq = positions, inv_freq
-    strides = positions.stride() if len(tokens) == 2 else (0, *positions.stride())
-    how.at = Positions(positions.data_ptr(), *strides)
-    batch = tokens[0] if len(tokens) == 2 else 1
-    how.shape = QkShape(batch, tokens[-1], q.shape[-2], k.shape[-2], dim, 2 * inv_freq.numel(), int(interleaved), dtype_code(q.dtype),
-                        dtype_code(weight_dtype), dtype_code(positions.dtype), eps)
+    batched = len(tokens) == 2
+    how.at = POSITIONS.pack(positions.data_ptr(), *(positions.stride() if batched else (0, positions.stride(0))))
+    try:
+        how.shape = QK_SHAPE.pack(tokens[0] if batched else 1, tokens[-1], x.q_heads, x.kv_heads, x.dim, rotary, int(interleaved), CODES[dtype],
+                                  CODES[weight_dtype], CODES[positions.dtype], eps)
+    except struct.error as e:
+        raise ValueError(f"qk_norm_rope: {e}") from None
     return how
-
-
-def _heads(t):
-    if t is None:
-        return HeadsView()
-    return HeadsView(t.data_ptr(), *(t.stride()[:-1] if t.dim() == 4 else (0, *t.stride()[:-1])))
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _qk_forward(q, k, q_weight, k_weight, how):
-    q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    k_out = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-    _call(q.device, lib().tdm_k6_qk_norm_rope, how.shape, _heads(q), _heads(k), _ptr(q_weight), _ptr(k_weight), how.at,
-          how.inv_freq.data_ptr(), _heads(q_out), _heads(k_out))
+def _qk_forward(like, q_weight, k_weight, x, how):
+    q_out = torch.empty(*x.tokens, x.q_heads, x.dim, device=like.device, dtype=like.dtype)
+    k_out = torch.empty(*x.tokens, x.kv_heads, x.dim, device=like.device, dtype=like.dtype)
+    _call(like, lib().tdm_k6_qk_norm_rope, how.shape, x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at, how.inv_freq.data_ptr(), _view(q_out), _view(k_out))
     return q_out, k_out
 
 
-def _upstream(g, like, what):
+def _upstream(g, x, heads, like, what):
     """An upstream gradient as the kernel reads it: of any strides, the last dimension contiguous."""
     if g is None:
         return None
-    if g.shape != like.shape or g.dtype != like.dtype or g.device != like.device:
-        raise ValueError(f"{what}: a gradient of {list(g.shape)} {g.dtype} on {g.device} for {list(like.shape)} {like.dtype} on {like.device}")
+    if g.dtype != like.dtype or list(g.shape) != [*x.tokens, heads, x.dim] or g.get_device() != like.get_device():
+        raise ValueError(f"{what}: a gradient of {list(g.shape)} {g.dtype} on {g.device} for {[*x.tokens, heads, x.dim]} {like.dtype} on {like.device}")
     return g if g.stride(-1) == 1 else g.contiguous()
 
 
-def _qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, how, dq, dk, dv):
-    dq_out, dk_out = _upstream(dq_out, q, "dq_out"), _upstream(dk_out, k, "dk_out")
-    dv_out = None if dv is None else _upstream(dv_out, dv, "dv_out")
+def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx):
+    dq_out, dk_out = _upstream(dq_out, x, x.q_heads, like, "dq_out"), _upstream(dk_out, x, x.kv_heads, like, "dk_out")
+    if dx.v is not None:
+        dv_out = _upstream(dv_out, x, x.kv_heads, like, "dv_out")
     L = lib()
     need = L.tdm_k6_qk_norm_rope_grad_workspace(how.shape)
-    if need < 0:
-        raise ValueError(L.tdm_last_error().decode(errors="replace"))
-    work = torch.empty(need, device=q.device, dtype=torch.uint8)
-    dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-    _call(q.device, L.tdm_k6_qk_norm_rope_grad, how.shape, _heads(dq_out), _heads(dk_out), _heads(dv_out), _heads(q), _heads(k),
-          _ptr(q_weight), _ptr(k_weight), how.at, how.inv_freq.data_ptr(), _heads(dq), _heads(dk), _heads(dv), _ptr(dqw), _ptr(dkw),
-          work.data_ptr(), need)
+    work = _workspace(need, like)
+    dqw, dkw = None if q_weight is None else torch.empty_like(q_weight), None if k_weight is None else torch.empty_like(k_weight)
+    _call(like, L.tdm_k6_qk_norm_rope_grad, how.shape, _view(dq_out), _view(dk_out), _view(dv_out), x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at,
+          how.inv_freq.data_ptr(), dx.q, dx.k, dx.v, _ptr(dqw), _ptr(dkw), work.data_ptr(), need)
     return dqw, dkw
+
+
+def _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how):
+    dq, dk = torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    dx = _Heads()
+    dx.q, dx.k, dx.v = _view(dq), _view(dk), None
+    return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, q_weight, k_weight, x, how, dx))
+
+
+def _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how):
+    dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
+    dx = _Heads()
+    dx.q_heads, dx.kv_heads, dx.dim = x.q_heads, x.kv_heads, x.dim
+    _place_packed(dx, dqkv)
+    return (dqkv, *_qk_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how, dx))
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, how):
+    def forward(ctx, q, k, q_weight, k_weight, x, how):
         ctx.save_for_backward(q, k, q_weight, k_weight, how.positions, how.inv_freq)
-        ctx.how = how
+        ctx.x, ctx.how = x, how
         ctx.set_materialize_grads(False)
-        return _qk_forward(q, k, q_weight, k_weight, how)
+        return _qk_forward(q, q_weight, k_weight, x, how)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight = ctx.saved_tensors[:4]
-        dq, dk = torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, k, q_weight, k_weight, ctx.how, dq, dk, None), None)
+        return (*_separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, ctx.x, ctx.how), None, None)
 
 
 class _QkvNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, q_heads, kv_heads, q_weight, k_weight, how):
+    def forward(ctx, qkv, q_weight, k_weight, x, how):
         ctx.save_for_backward(qkv, q_weight, k_weight, how.positions, how.inv_freq)
-        ctx.heads, ctx.how = (q_heads, kv_heads), how
+        ctx.x, ctx.how = x, how
         ctx.set_materialize_grads(False)
-        q, k, v = _split_qkv(qkv, q_heads, kv_heads)
-        return (*_qk_forward(q, k, q_weight, k_weight, how), v)
+        return (*_qk_forward(qkv, q_weight, k_weight, x, how), _values(qkv, x))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out, dv_out):
         qkv, q_weight, k_weight = ctx.saved_tensors[:3]
-        q, k, _ = _split_qkv(qkv, *ctx.heads)
-        dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
-        grads = _qk_backward(dq_out, dk_out, dv_out, q, k, q_weight, k_weight, ctx.how, *_split_qkv(dqkv, *ctx.heads))
-        return (dqkv, None, None, *grads, None)
+        return (*_packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, ctx.x, ctx.how), None, None)
 
 
 # ---- distillation from a teacher's top logits
@@ -349,8 +412,8 @@ def distill_loss(logits, teacher_index, teacher_logits, targets=None, temperatur
     gradient other than one (a loss that is scaled or divided afterwards) makes the backward pass compute it again."""
     how, operands = _check_distill(logits, teacher_index, teacher_logits, targets, temperature, weight, ignore_index, reduction, 1.0)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _Distill.apply(logits, *operands, how)
-    return _distill(logits, *operands, how, True, None, None, False)
+        return _Distill.apply(logits, *operands, how, reduction == "none")
+    return _distill(logits, *operands, how, reduction == "none", True, None, None, False)
 
 
 def distill_loss_and_grad(logits, teacher_index, teacher_logits, targets=None, temperature=1.0, weight=1.0, ignore_index=-100, reduction="mean",
@@ -360,7 +423,7 @@ def distill_loss_and_grad(logits, teacher_index, teacher_logits, targets=None, t
     the loss that is returned is not scaled. With reduction "none" the gradient is that of the sum."""
     how, operands = _check_distill(logits, teacher_index, teacher_logits, targets, temperature, weight, ignore_index, reduction, scale)
     grad = _empty_at_phase_of(logits)
-    return _distill(logits, *operands, how, True, grad, None, False), grad
+    return _distill(logits, *operands, how, reduction == "none", True, grad, None, False), grad
 
 
 def _empty_at_phase_of(t):
@@ -389,30 +452,31 @@ def _check_distill(logits, index, teacher, targets, temperature, weight, ignore_
         raise ValueError("a weight below 1 needs targets")
     _same_device(logits, index, teacher, targets)
     vocab = logits.shape[-1]
-    how = DistillHow(logits.numel() // vocab, vocab, ignore_index, teacher.shape[-1], dtype_code(logits.dtype), dtype_code(index.dtype),
-                     dtype_code(teacher.dtype), dtype_code(torch.int64 if targets is None else targets.dtype), REDUCTIONS[reduction],
-                     temperature, weight, scale)
+    try:
+        how = DISTILL_HOW.pack(logits.numel() // vocab, vocab, ignore_index, teacher.shape[-1], CODES[logits.dtype], CODES[index.dtype],
+                               CODES[teacher.dtype], CODES[torch.int64 if targets is None else targets.dtype], REDUCTIONS[reduction], temperature,
+                               weight, scale)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"distill_loss: {e}") from None
     return how, (index, teacher, targets)
 
 
-def _distill(logits, index, teacher, targets, how, want_loss, grad, upstream, keep_ones):
+def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, upstream, keep_ones):
     L = lib()
     need = L.tdm_k7_distill_workspace(how)
-    if need < 0:
-        raise ValueError(L.tdm_last_error().decode(errors="replace"))
-    work = torch.empty(need, device=logits.device, dtype=torch.uint8)
-    loss = torch.empty(logits.shape[:-1] if how.reduction == REDUCTIONS["none"] else (), device=logits.device) if want_loss else None
-    _call(logits.device, L.tdm_k7_distill, how, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), _ptr(targets), _ptr(loss), _ptr(grad),
+    work = _workspace(need, logits)
+    loss = torch.empty(logits.shape[:-1] if each_row else (), device=logits.device, dtype=torch.float32) if want_loss else None
+    _call(logits, L.tdm_k7_distill, how, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), _ptr(targets), _ptr(loss), _ptr(grad),
           _ptr(upstream), int(keep_ones), work.data_ptr(), need)
     return loss
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, index, teacher, targets, how):
+    def forward(ctx, logits, index, teacher, targets, how, each_row):
         ctx.save_for_backward(logits, index, teacher, targets)
-        ctx.how, ctx.grad = how, _empty_at_phase_of(logits)
-        return _distill(logits, index, teacher, targets, how, True, ctx.grad, None, False)
+        ctx.how, ctx.each_row, ctx.grad = how, each_row, _empty_at_phase_of(logits)
+        return _distill(logits, index, teacher, targets, how, each_row, True, ctx.grad, None, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -423,5 +487,5 @@ class _Distill(torch.autograd.Function):
         first = grad is not None
         if not first:
             grad = _empty_at_phase_of(ctx.saved_tensors[0])
-        _distill(*ctx.saved_tensors, ctx.how, False, grad, upstream.contiguous(), first)
-        return grad, None, None, None, None
+        _distill(*ctx.saved_tensors, ctx.how, ctx.each_row, False, grad, upstream.contiguous(), first)
+        return grad, None, None, None, None, None

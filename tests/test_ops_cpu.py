@@ -12,6 +12,20 @@ def _lib():
     return _lib
 
 
+def test_packed_structures_have_the_sizes_the_header_gives_them(tmp_path):
+    import os
+    import subprocess
+
+    source = tmp_path / "sizes.c"
+    source.write_text('#include "tandem_hip.h"\n#include <stdio.h>\nint main(void) { printf("%zu %zu %zu %zu", sizeof(tdm_heads), sizeof(tdm_positions), '
+                      'sizeof(tdm_qk_shape), sizeof(tdm_distill_how)); return 0; }\n')
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", include, str(source), "-o", str(tmp_path / "sizes")], check=True)
+    got = subprocess.run([str(tmp_path / "sizes")], stdout=subprocess.PIPE, text=True, check=True).stdout.split()
+    L = _lib()
+    assert [int(n) for n in got] == [s.size for s in (L.HEADS, L.POSITIONS, L.QK_SHAPE, L.DISTILL_HOW)]
+
+
 def refused(status, *words):
     message = _lib().lib().tdm_last_error().decode()
     assert status == 1 and all(w in message for w in words), (status, message)
@@ -64,25 +78,20 @@ def test_qk_norm_rope_refuses_cpu_tensors_and_odd_rotations():
 def test_qk_norm_rope_argument_errors_need_no_gpu():
     lib = _lib()
     L = lib.lib()
-    assert ctypes.sizeof(lib.HeadsView) == 32 and ctypes.sizeof(lib.Positions) == 24 and ctypes.sizeof(lib.QkShape) == 56
-
-    def shape(**change):
-        s = lib.QkShape(1, 2, 4, 2, 64, 64, 0, 3, 3, 4, 1e-6)
-        for name, value in change.items():
-            setattr(s, name, value)
-        return s
-
-    h, at, p = lib.HeadsView(4096, 128, 64, 64), lib.Positions(4096, 0, 1), ctypes.c_void_p(4096)  # never read
+    fields = dict(batch=1, tokens=2, q_heads=4, kv_heads=2, head_dim=64, rotary_dim=64, interleaved=0, dtype=3, weight_dtype=3, position_dtype=4, eps=1e-6)
+    shape = lambda **change: lib.QK_SHAPE.pack(*{**fields, **change}.values())  # noqa: E731
+    no_heads, no_positions = lib.HEADS.pack(0, 0, 0, 0), lib.POSITIONS.pack(0, 0, 0)
+    h, at, p = lib.HEADS.pack(4096, 128, 64, 64), lib.POSITIONS.pack(4096, 0, 1), ctypes.c_void_p(4096)  # never read
     call = lambda s, **k: L.tdm_k6_qk_norm_rope(s, k.get("q", h), h, p, p, k.get("at", at), k.get("freq", p), h, h, None)  # noqa: E731
     for change, word in ((dict(dtype=1), "dtype"), (dict(weight_dtype=2), "weights"), (dict(position_dtype=0), "positions"), (dict(tokens=1 << 31), "tokens"),
                          (dict(batch=-1), "tokens"), (dict(q_heads=-1), "heads"), (dict(head_dim=63), "even"), (dict(head_dim=514), "512"),
                          (dict(rotary_dim=66), "rotated"), (dict(rotary_dim=3), "rotated"), (dict(eps=-1.0), "eps")):
         refused(call(shape(**change)), word)
         assert L.tdm_k6_qk_norm_rope_grad_workspace(shape(**change)) == -1
-    refused(call(shape(), q=lib.HeadsView()), "null")
-    refused(call(shape(), at=lib.Positions()), "null")
+    refused(call(shape(), q=no_heads), "null")
+    refused(call(shape(), at=no_positions), "null")
     refused(call(shape(), freq=None), "null")
-    assert call(shape(tokens=0), q=lib.HeadsView()) == 0
+    assert call(shape(tokens=0), q=no_heads) == 0
     need = L.tdm_k6_qk_norm_rope_grad_workspace(shape())
     assert need >= 2 * 64 * 4
     grad = lambda w, n: L.tdm_k6_qk_norm_rope_grad(shape(), h, h, None, h, h, p, p, at, p, h, h, None, p, p, w, n, None)  # noqa: E731
@@ -101,13 +110,9 @@ def test_distill_loss_refuses_cpu_tensors():
 def test_distill_argument_errors_need_no_gpu():
     lib = _lib()
     L = lib.lib()
-    assert ctypes.sizeof(lib.DistillHow) == 64
-
-    def how(**change):
-        h = lib.DistillHow(4, 100, -100, 8, 0, 4, 0, 4, 1, 2.0, 1.0, 1.0)
-        for name, value in change.items():
-            setattr(h, name, value)
-        return h
+    fields = dict(rows=4, vocab=100, ignore_index=-100, k=8, dtype=0, index_dtype=4, teacher_dtype=0, target_dtype=4, reduction=1, temperature=2.0,
+                  weight=1.0, scale=1.0)
+    how = lambda **change: lib.DISTILL_HOW.pack(*{**fields, **change}.values())  # noqa: E731
 
     p, off = ctypes.c_void_p(4096), ctypes.c_void_p(4100)  # never read
     need = L.tdm_k7_distill_workspace(how())
