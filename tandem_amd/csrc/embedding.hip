@@ -69,8 +69,11 @@ __global__ __launch_bounds__(kLookupThreads) void embedding_lookup_kernel(Lookup
         const int64_t row = base + r * rows;
         const bool known = token[r] >= 0 && token[r] < a.vocab;
         const float scale = known ? a.scale : __builtin_nanf("");
+        float f[kN];
+        p[r].get(f);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) p[r].v[i] = narrow<T>(widen(p[r].v[i]) * scale);
+        for (int i = 0; i < kN; ++i) f[i] *= scale;
+        p[r].set(f);
         if (row < a.n) p[r].store_nt(static_cast<T*>(a.out) + row * a.dim + static_cast<int64_t>(v) * kN);
       }
     }
@@ -338,14 +341,15 @@ __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(SumArgs a) {
       float* to = a.partial + (chunk * 2 + (began_before ? 0 : 1)) * a.pitch + col;
 #pragma unroll
       for (int i = 0; i < kN; i += 4) {
-#pragma unroll
-        for (int j = 0; j < (kN < 4 ? kN : 4); ++j) p.v[j] = acc[i + j];
+        p.set(acc + i);
         p.store(to + i);
       }
     } else {
       P p;
+      float f[kN];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) p.v[i] = narrow<T>(acc[i] * a.scale);
+      for (int i = 0; i < kN; ++i) f[i] = acc[i] * a.scale;
+      p.set(f);
       p.store(static_cast<T*>(a.dweight) + static_cast<int64_t>(k) * a.dim + col);
     }
   };
@@ -369,8 +373,10 @@ __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(SumArgs a) {
 #pragma unroll
           for (int i = 0; i < kN; ++i) acc[i] = 0.0f;
         }
+        float f[kN];
+        row[u].get(f);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) acc[i] += widen(row[u].v[i]);
+        for (int i = 0; i < kN; ++i) acc[i] += f[i];
       }
     }
   }
@@ -399,17 +405,20 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void embedding_join_kernel(SumAr
   const int64_t per = (heads + kJoinWaves - 1) / kJoinWaves;
   const int64_t from = chunk + 1 + wave * per, to = std::min(chunk + 1 + heads, from + per);
   using P4 = Pack<float, 4>;
-  P4 acc{};
+  float acc[4] = {};
   if (col < a.dim) {
-    if (wave == 0) acc = P4::load(a.partial + (chunk * 2 + 1) * a.pitch + col);
+    if (wave == 0) P4::load(a.partial + (chunk * 2 + 1) * a.pitch + col).get(acc);
 #pragma unroll 8
     for (int64_t c = from; c < to; ++c) {
-      const P4 p = P4::load(a.partial + c * 2 * a.pitch + col);
+      float f[4];
+      P4::load(a.partial + c * 2 * a.pitch + col).get(f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc.v[i] += p.v[i];
+      for (int i = 0; i < 4; ++i) acc[i] += f[i];
     }
   }
-  acc.store(&s_acc[wave][lane * 4]);
+  P4 sums;
+  sums.set(acc);
+  sums.store(&s_acc[wave][lane * 4]);
   __syncthreads();
   const int64_t c = static_cast<int64_t>(blockIdx.y) * kJoinCols + threadIdx.x;
   if (c >= a.dim) return;

@@ -28,60 +28,70 @@ template <> struct RawOf<8> { typedef uint32_t type __attribute__((ext_vector_ty
 template <> struct RawOf<4> { typedef uint32_t type; };
 template <> struct RawOf<2> { typedef uint16_t type; };
 
+// kN elements that stay packed in their registers (element by element, 16-bit values take a register each).
 template <typename T, int kN>
 struct Pack {
   using raw_t = typename RawOf<kN * static_cast<int>(sizeof(T))>::type;
-  T v[kN];
-  static __device__ __forceinline__ Pack of(raw_t raw) {
-    Pack p;
-    __builtin_memcpy(&p, &raw, sizeof(raw));
-    return p;
+  raw_t raw;
+  static __device__ __forceinline__ Pack load(const T* at) { return Pack{*reinterpret_cast<const raw_t*>(at)}; }
+  static __device__ __forceinline__ Pack load_nt(const T* at) { return Pack{__builtin_nontemporal_load(reinterpret_cast<const raw_t*>(at))}; }
+  __device__ __forceinline__ void store(T* at) const { *reinterpret_cast<raw_t*>(at) = raw; }
+  __device__ __forceinline__ void store_nt(T* at) const { __builtin_nontemporal_store(raw, reinterpret_cast<raw_t*>(at)); }
+
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (kN * sizeof(T) == 2) {
+      f[0] = static_cast<float>(__builtin_bit_cast(T, raw));
+    } else {
+      constexpr int kWords = kN * static_cast<int>(sizeof(T)) / 4;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        uint32_t word;  // a copy: this compiler casts a vector's first element when given raw[i] itself
+        if constexpr (kWords == 1) word = raw;
+        else word = raw[i];
+        if constexpr (sizeof(T) == 4) {
+          f[i] = __uint_as_float(word);
+        } else {
+          typedef T pair __attribute__((ext_vector_type(2)));
+          typedef float pair32 __attribute__((ext_vector_type(2)));
+          const pair32 x = __builtin_convertvector(__builtin_bit_cast(pair, word), pair32);
+          f[2 * i] = x[0];
+          f[2 * i + 1] = x[1];
+        }
+      }
+    }
   }
-  static __device__ __forceinline__ Pack load(const T* at) { return of(*reinterpret_cast<const raw_t*>(at)); }
-  static __device__ __forceinline__ Pack load_nt(const T* at) { return of(__builtin_nontemporal_load(reinterpret_cast<const raw_t*>(at))); }
-  __device__ __forceinline__ raw_t raw() const {
-    raw_t r;
-    __builtin_memcpy(&r, this, sizeof(r));
-    return r;
+  __device__ __forceinline__ void set(const float* f) {
+    if constexpr (kN * sizeof(T) == 2) {
+      raw = __builtin_bit_cast(raw_t, static_cast<T>(f[0]));
+    } else {
+      constexpr int kWords = kN * static_cast<int>(sizeof(T)) / 4;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        uint32_t word;
+        if constexpr (sizeof(T) == 4) {
+          word = __float_as_uint(f[i]);
+        } else {
+          typedef T pair __attribute__((ext_vector_type(2)));
+          typedef float pair32 __attribute__((ext_vector_type(2)));
+          word = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair32{f[2 * i], f[2 * i + 1]}, pair));
+        }
+        if constexpr (kWords == 1) raw = word;
+        else raw[i] = word;
+      }
+    }
   }
-  __device__ __forceinline__ void store(T* at) const { *reinterpret_cast<raw_t*>(at) = raw(); }
-  __device__ __forceinline__ void store_nt(T* at) const { __builtin_nontemporal_store(raw(), reinterpret_cast<raw_t*>(at)); }
 };
 
-// 16 bytes of elements that stay packed in four registers (element by element, 16-bit values take a register each).
-typedef uint32_t Vec16 __attribute__((ext_vector_type(4)));
+typedef RawOf<16>::type Vec16;
 template <typename T>
 constexpr int per_vec() { return 16 / static_cast<int>(sizeof(T)); }
 template <typename T>
-__device__ __forceinline__ void unpack16(const Vec16& raw, float (&f)[per_vec<T>()]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(raw[i]);
-  } else {
-    typedef T pair __attribute__((ext_vector_type(2)));
-    typedef float pair32 __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t word = raw[i];  // a copy: this compiler casts the vector's first element when given raw[i] itself
-      const pair32 x = __builtin_convertvector(__builtin_bit_cast(pair, word), pair32);
-      f[2 * i] = x[0];
-      f[2 * i + 1] = x[1];
-    }
-  }
-}
+__device__ __forceinline__ void unpack16(const Vec16& raw, float (&f)[per_vec<T>()]) { Pack<T, per_vec<T>()>{raw}.get(f); }
 template <typename T>
 __device__ __forceinline__ Vec16 pack16(const float (&f)[per_vec<T>()]) {
-  Vec16 raw;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = __float_as_uint(f[i]);
-  } else {
-    typedef T pair __attribute__((ext_vector_type(2)));
-    typedef float pair32 __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair32{f[2 * i], f[2 * i + 1]}, pair));
-  }
-  return raw;
+  Pack<T, per_vec<T>()> p;
+  p.set(f);
+  return p.raw;
 }
 
 // A stretch of memory for buffer accesses: one register of offsets for many accesses (the rest of an address is scalar), loads
