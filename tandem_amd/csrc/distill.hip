@@ -411,6 +411,146 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
   }
 }
 
+// Short rows: 16 lanes a row, so that what a row needs once is done for four rows by every instruction of a wave (8192 rows of 256
+// floats, 16 entries, two temperatures: 14.1 us with a wave a row). kHeld vectors of the row and kEntries of the teacher's entries per lane.
+constexpr int kShortLanes = 16, kShortThreads = 256, kShortRows = kShortThreads / kShortLanes;
+
+template <typename T, int kHeld, int kEntries, bool kMix>
+__global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArgs a) {
+  constexpr int kN = per_vec<T>();
+  extern __shared__ uint32_t s_short[];  // k columns and k values of every row
+  const int sub = threadIdx.x % kShortLanes, place = threadIdx.x / kShortLanes;
+  uint32_t* const s_col = s_short + place * 2 * a.k;
+  float* const s_val = reinterpret_cast<float*>(s_col + a.k);
+  const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
+  const float inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = soft ? ck : kLog2e;
+  const float scale = a.scale / (a.count == nullptr ? a.divisor : *a.count);
+  const float lowest = -__builtin_inff();
+
+  const int64_t asked = static_cast<int64_t>(blockIdx.x) * kShortRows + place, row = std::min(asked, a.rows - 1);
+  const float up = a.upstream == nullptr ? 1.0f : a.upstream[row * a.upstream_step];
+  const int64_t y = a.targets == nullptr ? 0 : index_of(a.targets, a.targets_i64, row);
+  const bool skip = asked >= a.rows || (a.keep_ones && up == 1.0f), counted = a.targets == nullptr || y != a.ignore, live = !skip && counted;
+  const T* const x = static_cast<const T*>(a.logits) + row * a.vocab;
+  T* const g = static_cast<T*>(a.grad) + row * a.vocab;  // used where a.grad is given
+  const Body body = body_of(x, a.vocab);
+  const int edge = sub < body.head ? sub : sub - body.head < body.tail ? body.head + body.vecs * kN + sub - body.head : -1;
+
+  Vec16 held[kHeld];
+  float edge_x = lowest;
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (sub + i * kShortLanes < body.vecs) held[i] = reinterpret_cast<const Vec16*>(x + body.head)[sub + i * kShortLanes];
+    if (edge >= 0) edge_x = widen(x[edge]);
+  }
+  uint32_t col[kEntries];
+  float t[kEntries], x_col[kEntries], t_top = lowest, flags = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kEntries; ++i) {
+    col[i] = kNoColumn;
+    t[i] = lowest;
+    x_col[i] = 0.0f;
+    const int e = sub + i * kShortLanes;
+    if (!live || !soft || e >= a.k) continue;
+    const int64_t j = index_of(a.index, a.index_i64, row * a.k + e);
+    const float logit = teacher_logit(a, row * a.k + e);
+    if (j < 0) continue;
+    if (j >= a.vocab || logit != logit) {
+      flags = 1.0f;
+      continue;
+    }
+    col[i] = static_cast<uint32_t>(j);
+    t[i] = logit;
+    x_col[i] = widen(x[j]);
+    t_top = fmaxf(t_top, logit);
+  }
+  if (live && hard && (y < 0 || y >= a.vocab)) flags = 1.0f;
+  const bool bad = all_16(flags, Max{}) != 0.0f;
+  const float x_y = live && hard && !bad && sub == 0 ? widen(x[y]) : 0.0f;
+
+  Sums<kMix> sums;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (live && sub + i * kShortLanes < body.vecs) {
+      float f[kN];
+      unpack16<T>(held[i], f);
+      sums.take(f, c);
+    }
+  {
+    const float f[1] = {edge_x};
+    sums.take(f, c);
+  }
+  const float m = all_16(sums.m, Max{}), base = base_of(m);
+  sums.lift(m, c);
+  const float z = all_16(sums.z, Add{}), z1 = kMix ? all_16(sums.z1, Add{}) : z;
+  const float t_m = all_16(t_top, Max{});
+  float t_sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kEntries; ++i) t_sum += exp2_of((t[i] - base_of(t_m)) * ck);
+  const float t_z = all_16(t_sum, Add{});
+  const bool taught = soft && t_m != lowest, idle = !taught && !hard && !bad;
+  const float wrong = bad || (m == lowest && !idle) ? __builtin_nanf("") : 0.0f;
+
+  float p[kEntries], part = 0.0f;
+  bool mine = false;  // one of this lane's columns is the target
+#pragma unroll
+  for (int i = 0; i < kEntries; ++i) {
+    p[i] = 0.0f;
+    if (taught && col[i] != kNoColumn) {
+      const float tk = (t[i] - t_m) * inv_t;
+      p[i] = exp2_of(tk * kLog2e) / t_z;
+      if (!(p[i] == 0.0f)) part += a.weight * a.temperature * a.temperature * p[i] * (tk - ln_of(t_z) - ((x_col[i] - base) * inv_t - ln_of(z)));
+      mine = mine || (hard && col[i] == static_cast<uint32_t>(y));
+    }
+    const int e = sub + i * kShortLanes;
+    if (e < a.k) {
+      s_col[e] = col[i];
+      s_val[e] = p[i];
+    }
+  }
+  if (hard && sub == 0) part += (1.0f - a.weight) * (ln_of(z1) - (x_y - base));
+  part = all_16(part, Add{});
+  const bool covered = all_16(mine ? 1.0f : 0.0f, Max{}) != 0.0f;
+  if (a.rows_loss != nullptr && !skip && sub == 0) a.rows_loss[row] = counted ? part + wrong : 0.0f;
+  __syncthreads();
+  if (a.grad == nullptr || skip) return;
+
+  const float s = scale * up + wrong;
+  const float w_t = taught ? s * a.weight * a.temperature : wrong, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
+  const float k_t = (kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z), k_1 = kMix ? w_1 * __builtin_amdgcn_rcpf(z1) : 0.0f;
+  const bool zeros = !counted || idle;
+  auto slope = [&](float f) {
+    float e = k_t * exp2_of((f - base) * c);
+    if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
+    return e;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (sub + i * kShortLanes < body.vecs) {
+      Vec16 out = {0u, 0u, 0u, 0u};
+      if (!zeros) {
+        float f[kN];
+        unpack16<T>(held[i], f);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) f[e] = slope(f[e]);
+        out = pack16<T>(f);
+      }
+      reinterpret_cast<Vec16*>(g + body.head)[sub + i * kShortLanes] = out;
+    }
+  if (edge >= 0) g[edge] = narrow<T>(zeros ? 0.0f : slope(edge_x) + wrong);
+  if (zeros || bad) return;
+#pragma unroll
+  for (int i = 0; i < kEntries; ++i) {  // after the whole vectors, by the same wave
+    if (!taught || col[i] == kNoColumn) continue;
+    float down = 0.0f;
+    for (int e = 0; e < a.k; ++e) down += s_col[e] == col[i] ? w_t * s_val[e] : 0.0f;
+    if (hard && col[i] == static_cast<uint32_t>(y)) down += w_1;
+    g[col[i]] = narrow<T>(slope(x_col[i]) - down);
+  }
+  if (hard && sub == 0 && !covered) g[y] = narrow<T>(slope(x_y) - w_1);
+}
+
 constexpr int kFoldThreads = 1024;
 
 __device__ __forceinline__ float block_sum(float x) {
@@ -539,7 +679,14 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
           const integral_constant<int, 256> g256{};
           const integral_constant<int, 512> g512{};
           const integral_constant<int, 1024> g1024{};
-          if (h.k <= 64 && vecs <= 64) launch(g64, integral_constant<int, 1>{}, m);
+          auto launch_short = [&](auto held, auto entries) {
+            const unsigned bytes = static_cast<unsigned>(kShortRows * h.k * 8);
+            hipLaunchKernelGGL((distill_short_kernel<T, held.value, entries.value, m.value>), dim3(static_cast<unsigned>((h.rows + kShortRows - 1) / kShortRows)),
+                               dim3(kShortThreads), bytes, st, a);
+          };
+          if (h.k <= 16 && vecs <= 32) launch_short(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+          else if (h.k <= 16 && vecs <= 64) launch_short(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+          else if (h.k <= 64 && vecs <= 64) launch_short(integral_constant<int, 4>{}, integral_constant<int, 4>{});
           else if (h.k <= 64 && vecs <= 256) launch(g64, integral_constant<int, 4>{}, m);
           else if (h.k <= 256 && vecs <= 1024) launch(g256, integral_constant<int, 4>{}, m);
           else if (h.k <= 256 && vecs <= 2048) launch(g256, integral_constant<int, 8>{}, m);

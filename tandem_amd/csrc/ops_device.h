@@ -131,6 +131,14 @@ __device__ __forceinline__ float over_wave(float x, float none, F f) {
   x = dpp_step<0x143, 0xc>(x, none, f);
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
+// Over every row of 16 lanes, every lane gets it: neighbours, pairs, mirrored quads, mirrored eights.
+template <class F>
+__device__ __forceinline__ float all_16(float x, F f) {
+  x = dpp_step<0xb1, 0xf>(x, x, f);
+  x = dpp_step<0x4e, 0xf>(x, x, f);
+  x = dpp_step<0x141, 0xf>(x, x, f);
+  return dpp_step<0x140, 0xf>(x, x, f);
+}
 __device__ __forceinline__ float wave_sum(float x) { return over_wave(x, 0.0f, Add{}); }
 __device__ __forceinline__ float wave_max(float x) { return over_wave(x, -__builtin_inff(), Max{}); }
 
