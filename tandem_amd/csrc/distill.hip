@@ -32,10 +32,11 @@ struct DistillArgs {
   float* rows_loss;        // [rows]
   void* grad;              // null: not wanted
   const float* upstream;   // null: ones
-  const float* count;      // rows that count, the mean's divisor; null: `divisor`
+  const float* count;      // rows that count, the mean's divisor; null: counted by the workgroup itself, or `divisor`
   int64_t rows, vocab, ignore;
   int k, index_i64, teacher_dtype, targets_i64;
   int upstream_step;       // 0: one value for all rows
+  int counts;              // every workgroup counts the rows itself
   int keep_ones;           // where the upstream value is 1, the gradient there already is right
   float temperature, weight, scale, divisor;
 };
@@ -100,6 +101,15 @@ struct Sums {
   }
 };
 
+// This wave's part of the number of rows that count, kThreads lanes asking.
+template <int kThreads>
+__device__ __forceinline__ float counted_by_wave(const DistillArgs& a) {
+  float n = 0.0f;
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < a.rows; r += kThreads) n += index_of(a.targets, a.targets_i64, r) != a.ignore ? 1.0f : 0.0f;
+  return wave_sum(n);
+}
+
 // What a wave knows about a row, for the workgroup's others.
 struct WaveRow {
   float m, z, z1, t_m, t_z;
@@ -146,7 +156,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
   float* const s_val = reinterpret_cast<float*>(s_col + a.k);
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
-  const float inv_t = 1.0f / a.temperature, scale = a.scale / (a.count == nullptr ? a.divisor : *a.count);
+  const float inv_t = 1.0f / a.temperature;
   const float c = soft ? kLog2e * inv_t : kLog2e;  // without kMix: T where a = 1, else T = 1 or a = 0
 
   auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
@@ -211,7 +221,14 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) held[i] = load16<kStream>(from, lane16, i * kG * 16);
   }
+  if (a.counts) {
+    const float n = counted_by_wave<kG>(a);
+    if (lane == 0) s_part[0][wave] = n;
+  }
   __syncthreads();
+  const float counted = a.counts ? fmaxf(sum_of<kWaves>(s_part[0][lane % kWaves]), 1.0f) : a.count == nullptr ? a.divisor : *a.count;
+  const float scale = a.scale / counted;
+  __syncthreads();  // s_part is the rows' from here on
 
   for (int turn = 0; row < a.rows; turn ^= 1) {
     const T* const x = row_at(row);
@@ -420,11 +437,11 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
   constexpr int kN = per_vec<T>();
   extern __shared__ uint32_t s_short[];  // k columns and k values of every row
   const int sub = threadIdx.x % kShortLanes, place = threadIdx.x / kShortLanes;
+  __shared__ float s_count[kShortThreads / kWave];
   uint32_t* const s_col = s_short + place * 2 * a.k;
   float* const s_val = reinterpret_cast<float*>(s_col + a.k);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
   const float inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = soft ? ck : kLog2e;
-  const float scale = a.scale / (a.count == nullptr ? a.divisor : *a.count);
   const float lowest = -__builtin_inff();
 
   const int64_t asked = static_cast<int64_t>(blockIdx.x) * kShortRows + place, row = std::min(asked, a.rows - 1);
@@ -443,6 +460,10 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
     for (int i = 0; i < kHeld; ++i)
       if (sub + i * kShortLanes < body.vecs) held[i] = reinterpret_cast<const Vec16*>(x + body.head)[sub + i * kShortLanes];
     if (edge >= 0) edge_x = widen(x[edge]);
+  }
+  if (a.counts) {
+    const float n = counted_by_wave<kShortThreads>(a);
+    if (threadIdx.x % kWave == 0) s_count[threadIdx.x / kWave] = n;
   }
   uint32_t col[kEntries];
   float t[kEntries], x_col[kEntries], t_top = lowest, flags = 0.0f;
@@ -516,7 +537,16 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
   __syncthreads();
   if (a.grad == nullptr || skip) return;
 
-  const float s = scale * up + wrong;
+  float count = a.divisor;
+  if (a.counts) {
+    count = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kShortThreads / kWave; ++w) count += s_count[w];
+    count = fmaxf(count, 1.0f);
+  } else if (a.count != nullptr) {
+    count = *a.count;
+  }
+  const float s = a.scale / count * up + wrong;
   const float w_t = taught ? s * a.weight * a.temperature : wrong, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
   const float k_t = (kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z), k_1 = kMix ? w_1 * __builtin_amdgcn_rcpf(z1) : 0.0f;
   const bool zeros = !counted || idle;
@@ -553,29 +583,146 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
 
 constexpr int kFoldThreads = 1024;
 
-__device__ __forceinline__ float block_sum(float x) {
+// Of the waves' values (the same in all of a wave's lanes); every lane gets it.
+__device__ __forceinline__ float block_total(float of_wave) {
   __shared__ float s[kFoldThreads / kWave];
-  x = wave_sum(x);
-  if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = x;
   __syncthreads();
-  return wave_sum(threadIdx.x % kWave < kFoldThreads / kWave ? s[threadIdx.x % kWave] : 0.0f);
+  if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = of_wave;
+  __syncthreads();
+  return sum_of<kFoldThreads / kWave>(s[threadIdx.x % (kFoldThreads / kWave)]);
 }
 
 // How many rows count (at least one: a batch without any has loss 0).
-__global__ __launch_bounds__(kFoldThreads) void distill_count_kernel(const void* targets, int i64, int64_t rows, int64_t ignore, float* count) {
-  float n = 0.0f;
-#pragma unroll 8
-  for (int64_t r = threadIdx.x; r < rows; r += kFoldThreads) n += index_of(targets, i64, r) != ignore ? 1.0f : 0.0f;
-  n = block_sum(n);
+__global__ __launch_bounds__(kFoldThreads) void distill_count_kernel(DistillArgs a, float* count) {
+  const float n = block_total(counted_by_wave<kFoldThreads>(a));
   if (threadIdx.x == 0) *count = fmaxf(n, 1.0f);
 }
 
-__global__ __launch_bounds__(kFoldThreads) void distill_sum_kernel(const float* rows_loss, int64_t rows, const float* count, float divisor, float* loss) {
+__global__ __launch_bounds__(kFoldThreads) void distill_sum_kernel(DistillArgs a, float* loss) {
   float x = 0.0f;
 #pragma unroll 8
-  for (int64_t r = threadIdx.x; r < rows; r += kFoldThreads) x += rows_loss[r];
-  x = block_sum(x);
-  if (threadIdx.x == 0) *loss = x / (count == nullptr ? divisor : *count);
+  for (int64_t r = threadIdx.x; r < a.rows; r += kFoldThreads) x += a.rows_loss[r];
+  x = block_total(wave_sum(x));
+  const float n = a.counts ? fmaxf(block_total(counted_by_wave<kFoldThreads>(a)), 1.0f) : a.count == nullptr ? a.divisor : *a.count;
+  if (threadIdx.x == 0) *loss = x / n;
+}
+
+// The loss alone of a few long rows: with a workgroup per row most compute units are idle (4 rows of 131072 bf16 logits: 14.2 us and the
+// sum's launch). Every row is split over `slices` workgroups, which leave their maximum and sums; one more workgroup joins them, a wave
+// per row, with the teacher's share.
+constexpr int kSliceThreads = 256, kMostSlices = kWave;
+
+template <typename T, bool kMix>
+__global__ __launch_bounds__(kSliceThreads) void distill_slice_kernel(DistillArgs a, int slices, int per_slice, WaveRow* parts) {
+  constexpr int kN = per_vec<T>(), kWaves = kSliceThreads / kWave, kAhead = 4;
+  __shared__ WaveRow s_wave[kWaves];
+  const int64_t row = blockIdx.x / slices;
+  const int slice = blockIdx.x % slices, tid = threadIdx.x;
+  if (a.targets != nullptr && index_of(a.targets, a.targets_i64, row) == a.ignore) return;
+  const T* const x = static_cast<const T*>(a.logits) + row * a.vocab;
+  const Body body = body_of(x, a.vocab);
+  const float c = a.weight > 0.0f ? kLog2e / a.temperature : kLog2e;
+  Sums<kMix> sums;
+  if (slice == 0) {
+    const int edge = tid < body.head ? tid : tid - body.head < body.tail ? body.head + body.vecs * kN + tid - body.head : -1;
+    const float f[1] = {edge >= 0 ? widen(x[edge]) : -__builtin_inff()};
+    sums.take(f, c);
+  }
+  const Vec16* const from = reinterpret_cast<const Vec16*>(x + body.head);
+  const int end = std::min((slice + 1) * per_slice, body.vecs);
+  for (int v = slice * per_slice + tid; v < end; v += kSliceThreads * kAhead) {
+    Vec16 held[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v + u * kSliceThreads < end) held[u] = from[v + u * kSliceThreads];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v + u * kSliceThreads < end) {
+        float f[kN];
+        unpack16<T>(held[u], f);
+        sums.take(f, c);
+      }
+  }
+  WaveRow mine{};
+  mine.m = wave_max(sums.m);
+  sums.lift(mine.m, c);
+  mine.z = wave_sum(sums.z);
+  mine.z1 = kMix ? wave_sum(sums.z1) : mine.z;
+  if (tid % kWave == 0) s_wave[tid / kWave] = mine;
+  __syncthreads();
+  if (tid >= kWave) return;
+  const WaveRow w = s_wave[tid % kWaves];
+  Sums<kMix> part;
+  part.m = w.m;
+  part.z = w.z;
+  part.z1 = w.z1;
+  WaveRow all{};
+  all.m = max_of<kWaves>(w.m);
+  part.lift(all.m, c);
+  all.z = sum_of<kWaves>(part.z);
+  all.z1 = kMix ? sum_of<kWaves>(part.z1) : all.z;
+  if (tid == 0) parts[blockIdx.x] = all;
+}
+
+template <typename T, bool kMix>
+__global__ __launch_bounds__(kFoldThreads) void distill_slices_loss_kernel(DistillArgs a, int slices, const WaveRow* parts, float* loss, int each_row) {
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
+  const float lowest = -__builtin_inff(), inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = soft ? ck : kLog2e;
+  float total = 0.0f, count = 0.0f;
+  for (int64_t row = wave; row < a.rows; row += kFoldThreads / kWave) {
+    const int64_t y = a.targets == nullptr ? 0 : index_of(a.targets, a.targets_i64, row);
+    if (a.targets != nullptr && y == a.ignore) {
+      if (each_row && lane == 0) loss[row] = 0.0f;
+      continue;
+    }
+    const T* const x = static_cast<const T*>(a.logits) + row * a.vocab;
+    WaveRow w{};
+    if (lane < slices) w = parts[row * slices + lane];
+    else w.m = lowest;
+    Sums<kMix> part;
+    part.m = w.m;
+    part.z = w.z;
+    part.z1 = w.z1;
+    const float m = wave_max(w.m), base = base_of(m);
+    part.lift(m, c);
+    const float z = wave_sum(part.z), z1 = kMix ? wave_sum(part.z1) : z;
+    bool bad = hard && (y < 0 || y >= a.vocab);
+    auto entry = [&](int e, float& t) {  // its column, or -1
+      const int64_t j = index_of(a.index, a.index_i64, row * a.k + e);
+      t = teacher_logit(a, row * a.k + e);
+      if (j < 0) return int64_t(-1);
+      if (j < a.vocab && t == t) return j;
+      bad = true;
+      return int64_t(-1);
+    };
+    float t, t_top = lowest, t_sum = 0.0f, term = 0.0f;
+    for (int e = lane; soft && e < a.k; e += kWave)
+      if (entry(e, t) >= 0) t_top = fmaxf(t_top, t);
+    const float t_m = wave_max(t_top);
+    const bool taught = soft && t_m != lowest;
+    if (taught) {
+      for (int e = lane; e < a.k; e += kWave)
+        if (entry(e, t) >= 0) t_sum += exp2_of((t - t_m) * ck);
+      const float t_z = wave_sum(t_sum);
+      for (int e = lane; e < a.k; e += kWave) {
+        const int64_t j = entry(e, t);
+        const float tk = (t - t_m) * inv_t, p = j >= 0 ? exp2_of(tk * kLog2e) / t_z : 0.0f;
+        if (!(p == 0.0f)) term += a.weight * a.temperature * a.temperature * p * (tk - ln_of(t_z) - ((widen(x[j]) - base) * inv_t - ln_of(z)));
+      }
+    }
+    bad = __ballot(bad) != 0;
+    if (hard && !bad && lane == 0) term += (1.0f - a.weight) * (ln_of(z1) - (widen(x[y]) - base));
+    const bool idle = !taught && !hard && !bad;
+    const float row_loss = wave_sum(term) + (bad || (m == lowest && !idle) ? __builtin_nanf("") : 0.0f);
+    if (each_row && lane == 0) loss[row] = row_loss;
+    total += row_loss;
+    count += 1.0f;
+  }
+  if (each_row) return;
+  total = block_total(total);
+  count = block_total(count);
+  if (threadIdx.x == 0) *loss = total / (a.counts ? fmaxf(count, 1.0f) : a.divisor);
 }
 
 // ---------------------------------------------------------------- host
@@ -597,7 +744,14 @@ void check_how(const tdm_distill_how* h) {
 constexpr int64_t kCountBytes = 256;
 constexpr int kComputeUnits = 256;
 
-int64_t workspace_bytes_of(const tdm_distill_how& h) { return kCountBytes + (h.reduction == TDM_DISTILL_NONE ? 0 : h.rows * 4); }
+// Rows up to which every workgroup counts the targets itself (64 KiB of them from L2) instead of a launch that does.
+constexpr int64_t kCountRows = 8192;
+// Rows up to which the loss alone of long rows is split over the rows' length: the joining workgroup has a wave for two of them.
+constexpr int64_t kSlicedRows = 32;
+
+int64_t workspace_bytes_of(const tdm_distill_how& h) {
+  return kCountBytes + std::max<int64_t>(h.reduction == TDM_DISTILL_NONE ? 0 : h.rows * 4, h.rows <= kSlicedRows ? h.rows * kMostSlices * static_cast<int64_t>(sizeof(WaveRow)) : 0);
+}
 
 }  // namespace
 
@@ -634,10 +788,6 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
     float* const count = static_cast<float*>(workspace);
     float* const rows_loss = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes);
     const bool mean = h.reduction == TDM_DISTILL_MEAN;
-    if (mean && targets != nullptr) {
-      hipLaunchKernelGGL(distill_count_kernel, dim3(1), dim3(kFoldThreads), 0, st, targets, h.target_dtype == TDM_I64, h.rows, h.ignore_index, count);
-      check_launch("distill_count launch");
-    }
     DistillArgs a{};
     a.logits = logits;
     a.index = teacher_index;
@@ -646,7 +796,7 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
     a.rows_loss = loss == nullptr ? nullptr : h.reduction == TDM_DISTILL_NONE ? loss : rows_loss;
     a.grad = grad;
     a.upstream = upstream;
-    a.count = mean && targets != nullptr ? count : nullptr;
+    a.counts = mean && targets != nullptr;
     a.divisor = mean ? static_cast<float>(std::max<int64_t>(h.rows, 1)) : 1.0f;
     a.rows = h.rows;
     a.vocab = h.vocab;
@@ -660,6 +810,30 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
     a.temperature = h.temperature;
     a.weight = h.weight;
     a.scale = h.scale;
+    const int64_t all_vecs = h.vocab * (h.dtype == TDM_F32 ? 4 : 2) / 16;
+    if (grad == nullptr && h.rows > 0 && h.rows <= kSlicedRows && all_vecs > 2048) {
+      const int slices = static_cast<int>(std::min<int64_t>(kMostSlices, std::min<int64_t>((all_vecs + 1023) / 1024, 512 / h.rows)));
+      const int per_slice = static_cast<int>((all_vecs + slices - 1) / slices);
+      WaveRow* const parts = reinterpret_cast<WaveRow*>(rows_loss);
+      with_dtype(h.dtype, [&](auto t) {
+        using T = decltype(t);
+        auto launch = [&](auto m) {
+          hipLaunchKernelGGL((distill_slice_kernel<T, m.value>), dim3(static_cast<unsigned>(h.rows * slices)), dim3(kSliceThreads), 0, st, a, slices, per_slice, parts);
+          check_launch("distill_slice launch");
+          hipLaunchKernelGGL((distill_slices_loss_kernel<T, m.value>), dim3(1), dim3(kFoldThreads), 0, st, a, slices, parts, loss, h.reduction == TDM_DISTILL_NONE);
+          check_launch("distill_slices_loss launch");
+        };
+        if (h.weight > 0.0f && h.weight < 1.0f && h.temperature != 1.0f) launch(std::true_type{});
+        else launch(std::false_type{});
+      });
+      return;
+    }
+    if (a.counts && (h.rows > kCountRows || (h.k <= 64 && all_vecs > 64 && all_vecs <= 256))) {  // a workgroup of one wave does not count
+      hipLaunchKernelGGL(distill_count_kernel, dim3(1), dim3(kFoldThreads), 0, st, a, count);
+      check_launch("distill_count launch");
+      a.counts = 0;
+      a.count = count;
+    }
     if (h.rows > 0) {
       const bool mix = h.weight > 0.0f && h.weight < 1.0f && h.temperature != 1.0f;
       int log_table = 6;  // at most half full
@@ -701,7 +875,7 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
       check_launch("distill launch");
     }
     if (loss != nullptr && h.reduction != TDM_DISTILL_NONE) {
-      hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kFoldThreads), 0, st, rows_loss, h.rows, a.count, a.divisor, loss);
+      hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(kFoldThreads), 0, st, a, loss);
       check_launch("distill_sum launch");
     }
   });
