@@ -384,8 +384,8 @@ __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(SumArgs a) {
 }
 
 // A workgroup per chunk and slice of 256 columns: if a token begins in the chunk and goes on behind it, its partial sums, the
-// workgroup's four waves a quarter of them each.
-constexpr int kJoinWaves = 4;
+// workgroup's waves an eighth of them each.
+constexpr int kJoinWaves = 8;
 constexpr int kJoinCols = 4 * kWave;
 
 template <typename T>
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void embedding_join_kernel(SumAr
   sums.store(&s_acc[wave][lane * 4]);
   __syncthreads();
   const int64_t c = static_cast<int64_t>(blockIdx.y) * kJoinCols + threadIdx.x;
-  if (c >= a.dim) return;
+  if (threadIdx.x >= kJoinCols || c >= a.dim) return;
   float sum = s_acc[0][threadIdx.x];
 #pragma unroll
   for (int w = 1; w < kJoinWaves; ++w) sum += s_acc[w][threadIdx.x];
@@ -437,7 +437,7 @@ constexpr int64_t kMostVocab = int64_t(1) << 24;  // 2^14 workgroups place the t
 // Entries of a chunk: 64, or fewer as long as there are fewer than 2048 waves of 512 columns.
 int chunk_of(int64_t n, int64_t dim) {
   int chunk = 64;
-  while (chunk > 8 && n / chunk * ((dim + 511) / 512) < 2048) chunk /= 2;
+  while (chunk > 16 && n / chunk * ((dim + 511) / 512) < 2048) chunk /= 2;
   return chunk;
 }
 

@@ -7,6 +7,11 @@ the data-parallel path can observe: module names, parameter registration order
 and shapes, the seeded initialisation (same draws in the same order), presets
 and units(). The kernels here never look inside the model; it defines the shapes
 of every gradient, bucket, shard and unit in the benchmarks.
+
+Beyond the reference, and off by default: a model whose queries and keys are normed
+per head and rotated by position (Config.rotary, with no position table), whose
+token embedding is scaled (Config.embed_scale), and whose loss is a teacher's
+(GPT.forward's `teacher`). These run on the kernels of tandem_amd.ops, on the GPU only.
 """
 
 import math
@@ -15,6 +20,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from . import ops
 
 _PRESETS = {
     "tiny": {},
@@ -31,6 +38,12 @@ class Config:
     layers: int = 4
     heads: int = 4
     dim: int = 128
+    rotary: bool = False  # queries and keys normed per head and rotated by position; no position table
+    embed_scale: float = 1.0  # of the token embedding; only with rotary
+
+    def __post_init__(self):
+        if self.embed_scale != 1.0 and not self.rotary:
+            raise ValueError("embed_scale needs rotary=True")
 
     @staticmethod
     def preset(name):
@@ -43,9 +56,26 @@ class Attention(nn.Module):
         self.heads = cfg.heads
         self.qkv = nn.Linear(cfg.dim, 3 * cfg.dim)
         self.proj = nn.Linear(cfg.dim, cfg.dim)
+        self.rotary = cfg.rotary
+        if cfg.rotary:
+            self.q_norm = nn.Parameter(torch.ones(cfg.dim // cfg.heads))
+            self.k_norm = nn.Parameter(torch.ones(cfg.dim // cfg.heads))
+            self._seq, self._turn = cfg.seq, {}
+
+    def _rotation(self, device):
+        """(positions 0 .. seq - 1, angles per position) on `device`; not buffers, which a cast of the model would round."""
+        if device not in self._turn:
+            per_head = self.q_norm.shape[0]
+            self._turn[device] = (torch.arange(self._seq, device=device), ops.rope_frequencies(per_head, device=device))
+        return self._turn[device]
 
     def forward(self, x):
         batch, steps, width = x.shape
+        if self.rotary:
+            positions, inv_freq = self._rotation(x.device)
+            heads = ops.qkv_norm_rope(self.qkv(x), self.heads, self.heads, self.q_norm, self.k_norm, positions[:steps], inv_freq)
+            mixed = F.scaled_dot_product_attention(*(part.transpose(1, 2) for part in heads), is_causal=True)
+            return self.proj(mixed.transpose(1, 2).reshape(batch, steps, width))
         per_head = width // self.heads
         q, k, v = (part.view(batch, steps, self.heads, per_head).transpose(1, 2)
                    for part in self.qkv(x).split(width, dim=2))
@@ -71,9 +101,12 @@ class Embed(nn.Module):
     def __init__(self, cfg):
         super().__init__()
         self.tok = nn.Embedding(cfg.vocab, cfg.dim)
-        self.pos = nn.Embedding(cfg.seq, cfg.dim)
+        self.scale = cfg.embed_scale
+        self.pos = None if cfg.rotary else nn.Embedding(cfg.seq, cfg.dim)
 
     def forward(self, idx):
+        if self.pos is None:
+            return ops.embedding(idx, self.tok.weight, scale=self.scale)
         where = torch.arange(idx.shape[1], device=idx.device)
         return self.tok(idx) + self.pos(where)
 
@@ -113,11 +146,15 @@ class GPT(nn.Module):
         """The model as a sequence of modules: what ZeRO-3 shards one at a time."""
         return [self.embed, *self.blocks, self.head]
 
-    def forward(self, idx, targets=None):
+    def forward(self, idx, targets=None, teacher=None, temperature=1.0, teacher_weight=1.0):
+        """The logits; with `targets` the loss. `teacher`: (columns, logits) of a teacher's top logits, each [batch, tokens, k]; the
+        loss is then ops.distill_loss of them at `temperature`, mixed with the targets' share 1 - teacher_weight."""
         x = self.embed(idx)
         for block in self.blocks:
             x = block(x)
         logits = self.head(x)
+        if teacher is not None:
+            return ops.distill_loss(logits, *teacher, targets=targets, temperature=temperature, weight=teacher_weight)
         return logits if targets is None else loss_fn(logits, targets)
 
 

@@ -272,7 +272,18 @@ def _wants_grad(w):
 class _QkHow:
     """What a call and its gradient share besides the tensors they differentiate."""
 
-    __slots__ = ("shape", "positions", "at", "inv_freq")
+    __slots__ = ("shape", "positions", "inv_freq")
+
+    def at(self):
+        """The positions as tdm_positions."""
+        strides = self.positions.stride()
+        return POSITIONS.pack(self.positions.data_ptr(), *(strides if len(strides) == 2 else (0, strides[0])))
+
+    def of(self, positions, inv_freq):
+        """The same call on the tensors that the backward pass got back: hooks on saved tensors may have moved them."""
+        how = _QkHow()
+        how.shape, how.positions, how.inv_freq = self.shape, positions, inv_freq
+        return how
 
 
 def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved):
@@ -300,10 +311,8 @@ def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved
             raise ValueError(f"positions of {list(positions.shape)} for tokens of {tokens}") from None
     how = _QkHow()
     how.positions, how.inv_freq = positions, inv_freq
-    batched = len(tokens) == 2
-    how.at = POSITIONS.pack(positions.data_ptr(), *(positions.stride() if batched else (0, positions.stride(0))))
     try:
-        how.shape = QK_SHAPE.pack(tokens[0] if batched else 1, tokens[-1], x.q_heads, x.kv_heads, x.dim, rotary, int(interleaved), CODES[dtype],
+        how.shape = QK_SHAPE.pack(tokens[0] if len(tokens) == 2 else 1, tokens[-1], x.q_heads, x.kv_heads, x.dim, rotary, int(interleaved), CODES[dtype],
                                   CODES[weight_dtype], CODES[positions.dtype], eps)
     except struct.error as e:
         raise ValueError(f"qk_norm_rope: {e}") from None
@@ -317,7 +326,7 @@ def _ptr(t):
 def _qk_forward(like, q_weight, k_weight, x, how):
     q_out = torch.empty(*x.tokens, x.q_heads, x.dim, device=like.device, dtype=like.dtype)
     k_out = torch.empty(*x.tokens, x.kv_heads, x.dim, device=like.device, dtype=like.dtype)
-    _call(like, lib().tdm_k6_qk_norm_rope, how.shape, x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at, how.inv_freq.data_ptr(), _view(q_out), _view(k_out))
+    _call(like, lib().tdm_k6_qk_norm_rope, how.shape, x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at(), how.inv_freq.data_ptr(), _view(q_out), _view(k_out))
     return q_out, k_out
 
 
@@ -338,7 +347,7 @@ def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx):
     need = L.tdm_k6_qk_norm_rope_grad_workspace(how.shape)
     work = _workspace(need, like)
     dqw, dkw = None if q_weight is None else torch.empty_like(q_weight), None if k_weight is None else torch.empty_like(k_weight)
-    _call(like, L.tdm_k6_qk_norm_rope_grad, how.shape, _view(dq_out), _view(dk_out), _view(dv_out), x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at,
+    _call(like, L.tdm_k6_qk_norm_rope_grad, how.shape, _view(dq_out), _view(dk_out), _view(dv_out), x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at(),
           how.inv_freq.data_ptr(), dx.q, dx.k, dx.v, _ptr(dqw), _ptr(dkw), work.data_ptr(), need)
     return dqw, dkw
 
@@ -362,30 +371,30 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, x, how):
         ctx.save_for_backward(q, k, q_weight, k_weight, how.positions, how.inv_freq)
-        ctx.x, ctx.how = x, how
+        ctx.how = how.of(None, None)
         ctx.set_materialize_grads(False)
         return _qk_forward(q, q_weight, k_weight, x, how)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
-        q, k, q_weight, k_weight = ctx.saved_tensors[:4]
-        return (*_separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, ctx.x, ctx.how), None, None)
+        q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+        return (*_separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, _separate(q, k), ctx.how.of(positions, inv_freq)), None, None)
 
 
 class _QkvNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, x, how):
         ctx.save_for_backward(qkv, q_weight, k_weight, how.positions, how.inv_freq)
-        ctx.x, ctx.how = x, how
+        ctx.heads, ctx.how = (x.q_heads, x.kv_heads), how.of(None, None)
         ctx.set_materialize_grads(False)
         return (*_qk_forward(qkv, q_weight, k_weight, x, how), _values(qkv, x))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out, dv_out):
-        qkv, q_weight, k_weight = ctx.saved_tensors[:3]
-        return (*_packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, ctx.x, ctx.how), None, None)
+        qkv, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
+        return (*_packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, _packed(qkv, *ctx.heads), ctx.how.of(positions, inv_freq)), None, None)
 
 
 # ---- distillation from a teacher's top logits

@@ -135,3 +135,20 @@ def test_distill_argument_errors_need_no_gpu():
     refused(call(how(), nbytes=need - 1), "workspace")
     refused(call(how(), work=off), "workspace")
     refused(call(how(), grad=off), "16-byte")
+
+
+def test_the_rotary_model_s_parameters_and_refusals():
+    from tandem_amd.model import GPT, Config
+
+    cfg = Config(seq=16, layers=1, heads=2, dim=16, rotary=True, embed_scale=4.0)
+    model = GPT(cfg)
+    names = [n for n, _ in model.named_parameters()]
+    assert "embed.pos.weight" not in names and "blocks.0.attn.q_norm" in names and model.blocks[0].attn.q_norm.shape == (8,)
+    assert [n for n, _ in GPT(Config(seq=16, layers=1, heads=2, dim=16)).named_parameters()][:2] == ["embed.tok.weight", "embed.pos.weight"]
+    with pytest.raises(ValueError, match="no CPU path"):
+        model(torch.zeros(1, 4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="rotary"):
+        Config(embed_scale=2.0)
+    plain = GPT(Config(seq=16, layers=1, heads=2, dim=16))
+    with pytest.raises(ValueError, match="no CPU path"):
+        plain(torch.zeros(1, 4, dtype=torch.int64), teacher=(torch.zeros(1, 4, 2, dtype=torch.int64), torch.zeros(1, 4, 2)))
