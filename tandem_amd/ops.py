@@ -50,7 +50,7 @@ def _same_device(first, *others):
 def _call(t, entry, *args):
     """entry(*args, stream) on the current stream of `t`'s device: the launch goes to the current device, which may be another."""
     device = t.get_device()
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -62,7 +62,18 @@ def _call(t, entry, *args):
 def _workspace(bytes_needed, like):
     if bytes_needed < 0:
         raise ValueError(lib().tdm_last_error().decode(errors="replace"))
-    return torch.empty(bytes_needed, device=like.device, dtype=torch.uint8)
+    return like.new_empty(bytes_needed, dtype=torch.uint8)
+
+
+def _once(backward):
+    """torch's once_differentiable, which runs the backward pass without gradients and refuses a second one, where a second one was asked for
+    (only then do gradients flow in a backward pass): its own bookkeeping costs more than most launches."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 # ---- embedding
@@ -100,7 +111,7 @@ def _embedding(tokens, weight, scale):
     tokens = _indices(tokens, "embedding(tokens)")
     _same_device(weight, tokens)
     vocab, dim = weight.shape
-    out = torch.empty(*tokens.shape, dim, device=weight.device, dtype=weight.dtype)
+    out = weight.new_empty((*tokens.shape, dim))
     _call(weight, lib().tdm_k5_embedding, weight.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), tokens.numel(), vocab, dim,
           CODES[weight.dtype], scale)
     return out
@@ -123,7 +134,7 @@ def _embedding_grad(grad, tokens, vocab, scale, padding):
     if grad.dim() < 1 or grad.shape[:-1] != tokens.shape or grad.shape[-1] == 0:
         raise ValueError(f"embedding_grad: a gradient of {list(grad.shape)} for tokens of {list(tokens.shape)}")
     n, dim = tokens.numel(), grad.shape[-1]
-    out = torch.empty(vocab, dim, device=grad.device, dtype=grad.dtype)
+    out = grad.new_empty((vocab, dim))
     L = lib()
     need = L.tdm_k5_embedding_grad_workspace(n, vocab, dim)
     work = _workspace(need, grad)
@@ -141,7 +152,7 @@ class _Embedding(torch.autograd.Function):
         return _embedding(tokens, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
         return None, _embedding_grad(grad.contiguous(), tokens, *ctx.how), None, None
@@ -324,8 +335,7 @@ def _ptr(t):
 
 
 def _qk_forward(like, q_weight, k_weight, x, how):
-    q_out = torch.empty(*x.tokens, x.q_heads, x.dim, device=like.device, dtype=like.dtype)
-    k_out = torch.empty(*x.tokens, x.kv_heads, x.dim, device=like.device, dtype=like.dtype)
+    q_out, k_out = like.new_empty((*x.tokens, x.q_heads, x.dim)), like.new_empty((*x.tokens, x.kv_heads, x.dim))
     _call(like, lib().tdm_k6_qk_norm_rope, how.shape, x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at(), how.inv_freq.data_ptr(), _view(q_out), _view(k_out))
     return q_out, k_out
 
@@ -353,14 +363,14 @@ def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx):
 
 
 def _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how):
-    dq, dk = torch.empty(q.shape, device=q.device, dtype=q.dtype), torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     dx = _Heads()
     dx.q, dx.k, dx.v = _view(dq), _view(dk), None
     return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, q_weight, k_weight, x, how, dx))
 
 
 def _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how):
-    dqkv = torch.empty(qkv.shape, device=qkv.device, dtype=qkv.dtype)
+    dqkv = qkv.new_empty(qkv.shape)
     dx = _Heads()
     dx.q_heads, dx.kv_heads, dx.dim = x.q_heads, x.kv_heads, x.dim
     _place_packed(dx, dqkv)
@@ -376,7 +386,7 @@ class _QkNormRope(torch.autograd.Function):
         return _qk_forward(q, q_weight, k_weight, x, how)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
         return (*_separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, _separate(q, k), ctx.how.of(positions, inv_freq)), None, None)
@@ -391,7 +401,7 @@ class _QkvNormRope(torch.autograd.Function):
         return (*_qk_forward(qkv, q_weight, k_weight, x, how), _values(qkv, x))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq_out, dk_out, dv_out):
         qkv, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
         return (*_packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, _packed(qkv, *ctx.heads), ctx.how.of(positions, inv_freq)), None, None)
@@ -439,8 +449,8 @@ def _empty_at_phase_of(t):
     """An uninitialised contiguous tensor like `t` that starts at the same distance from a 16-byte boundary."""
     lead = t.data_ptr() % 16 // t.element_size()
     if lead == 0:
-        return torch.empty(t.shape, device=t.device, dtype=t.dtype)
-    return torch.empty(t.numel() + lead, device=t.device, dtype=t.dtype)[lead:].view(t.shape)
+        return t.new_empty(t.shape)
+    return t.new_empty(t.numel() + lead)[lead:].view(t.shape)
 
 
 def _check_distill(logits, index, teacher, targets, temperature, weight, ignore_index, reduction, scale):
@@ -474,7 +484,7 @@ def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, up
     L = lib()
     need = L.tdm_k7_distill_workspace(how)
     work = _workspace(need, logits)
-    loss = torch.empty(logits.shape[:-1] if each_row else (), device=logits.device, dtype=torch.float32) if want_loss else None
+    loss = logits.new_empty(logits.shape[:-1] if each_row else (), dtype=torch.float32) if want_loss else None
     _call(logits, L.tdm_k7_distill, how, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), _ptr(targets), _ptr(loss), _ptr(grad),
           _ptr(upstream), int(keep_ones), work.data_ptr(), need)
     return loss
@@ -488,7 +498,7 @@ class _Distill(torch.autograd.Function):
         return _distill(logits, index, teacher, targets, how, each_row, True, ctx.grad, None, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, upstream):
         # the gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out
         # once; a second backward pass through the same graph computes its own.

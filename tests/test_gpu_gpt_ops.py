@@ -234,3 +234,17 @@ def test_the_strategies_agree_on_the_rotary_model():
     for ranks in runs.values():
         assert [r[0] for r in ranks] == losses
         assert all(torch.equal(r[1], weights) for r in ranks)
+
+
+def test_a_second_derivative_is_refused():
+    from tandem_amd import ops
+
+    w = torch.randn(10, 16, device=DEV, requires_grad=True)
+    x = torch.randn(4, 30, device=DEV, requires_grad=True)
+    columns, logits = torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.randn(4, 2, device=DEV)
+    qkv = torch.randn(5, 48, device=DEV, requires_grad=True)
+    q, _, _ = ops.qkv_norm_rope(qkv, 1, 1, None, None, torch.arange(5, device=DEV), ops.rope_frequencies(16))
+    for out, leaf in ((ops.embedding(torch.arange(4, device=DEV), w), w), (ops.distill_loss(x, columns, logits), x), (q, qkv)):
+        (first,) = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
