@@ -7,7 +7,8 @@
 // the order of n), then the rows of g are read once each in that order and added in fp32 registers; a row of dW is written
 // once, rounded once. No float atomics: the order of every sum is fixed by n, the vocabulary and the width alone.
 //
-//   1. embedding_sort_kernel: every workgroup reads all tokens and places those of its share of the vocabulary.
+//   1. embedding_sort_kernel: every workgroup reads all tokens and places those of its share of the vocabulary. Of more than 8192 tokens
+//      embedding_split_kernel first brings those of a share together, 1024 at a time, and embedding_place_kernel reads its own.
 //   2. embedding_sum_kernel: a wave takes a chunk of the sorted entries and a slice of the columns. A token whose entries all lie in
 //      the chunk is finished there; one that crosses the chunk's ends leaves fp32 partial sums. The launch's other workgroups
 //      write the zeros of the rows that have no token (most rows of a large vocabulary).
@@ -116,6 +117,14 @@ __device__ __forceinline__ uint32_t key_of(const SortArgs& a, uint32_t n) {
   return fits && low < a.vocab && low != a.padding ? low : kNoToken;
 }
 
+// The zeros that a sort's launch writes beside it.
+template <int kThreads>
+__device__ __forceinline__ void write_zeros(void* base, int64_t bytes, int64_t block, int64_t blocks) {
+  const Vec16 none = {0u, 0u, 0u, 0u};
+  Vec16* const to = static_cast<Vec16*>(base);
+  for (int64_t v = block * kThreads + threadIdx.x; v < bytes / 16; v += blocks * kThreads) __builtin_nontemporal_store(none, to + v);
+}
+
 // Counting sort, a workgroup per share of the vocabulary. Every workgroup reads all tokens (they stay in L2): first it counts those
 // of lower shares and, per wave and token, those of its own; after a sum over tokens and waves it knows where each wave's entries
 // of each token go, and places them in the order in which they come: a wave walks its stretch of tokens 64 at a
@@ -126,11 +135,8 @@ __device__ __forceinline__ uint32_t key_of(const SortArgs& a, uint32_t n) {
 template <typename I, int kHeld>
 __global__ __launch_bounds__(kSortThreads, 8) void embedding_sort_kernel(SortArgs a) {
   if (blockIdx.x >> a.log_shares != 0) {
-    typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
-    const vec16 none = {0u, 0u, 0u, 0u};
-    vec16* const to = static_cast<vec16*>(a.zero);
-    const int64_t blocks = static_cast<int64_t>(gridDim.x) - (int64_t(1) << a.log_shares);
-    for (int64_t v = (blockIdx.x - (int64_t(1) << a.log_shares)) * kSortThreads + threadIdx.x; v < a.zero_bytes / 16; v += blocks * kSortThreads) __builtin_nontemporal_store(none, to + v);
+    const int64_t shares = int64_t(1) << a.log_shares;
+    write_zeros<kSortThreads>(a.zero, a.zero_bytes, blockIdx.x - shares, gridDim.x - shares);
     return;
   }
   extern __shared__ uint32_t s_count[];  // [waves][share]
@@ -236,6 +242,204 @@ __global__ __launch_bounds__(kSortThreads, 8) void embedding_sort_kernel(SortArg
   }
 }
 
+// The same result for many tokens, each read by one workgroup instead of by all (32768 int64 tokens of a vocabulary of 131072: 25 us by 256
+// workgroups that all read them, most of it waiting for the same lines). A tile of tokens is brought in order of their shares, `from`
+// where they came from; offsets[tile][share]: where the share's begin in the tile.
+constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / kWave, kSplitItems = 2, kTile = kSplitThreads * kSplitItems;
+constexpr int kPlaceItems = 4;
+constexpr int64_t kOneLaunch = 8192;  // tokens that the one launch is quicker with
+constexpr int kMostTiles = 1024;  // a workgroup that places holds their numbers in LDS
+
+struct SplitArgs {
+  SortArgs sort;
+  uint32_t *numbers, *from;  // [n] the token's number in its share; where it stood
+  uint32_t* offsets;         // [tiles][shares + 1]
+  int tiles, number_bits;
+};
+
+// The lanes that hold the same value (of `bits` bits) as this one, among those that take part.
+__device__ __forceinline__ uint64_t lanes_like(uint32_t value, int bits, bool takes_part) {
+  uint64_t same = __ballot(takes_part);
+  for (int b = 0; b < bits; ++b) {
+    const bool on = (value >> b) & 1;
+    const uint64_t votes = __ballot(on);
+    same &= on ? votes : ~votes;
+  }
+  return same;
+}
+
+// Moves the wave's counter of `value` on by the lanes that hold it; every one of them gets its own place: they stay in order.
+__device__ __forceinline__ uint32_t claim(uint32_t* count, uint32_t value, int bits, bool takes_part) {
+  const uint32_t lane = threadIdx.x % kWave;
+  const uint64_t same = lanes_like(value, bits, takes_part);
+  const int leader = takes_part ? __builtin_ctzll(same) : 0;
+  uint32_t found = 0;
+  if (takes_part && lane == static_cast<uint32_t>(leader)) found = atomicAdd(&count[value], static_cast<uint32_t>(__popcll(same)));
+  return __shfl(found, leader) + static_cast<uint32_t>(__popcll(same & ((1ull << lane) - 1)));
+}
+
+// s_count [waves][width], the number of every wave's entries of every value, becomes where they begin, from `begin` on; returns where
+// this lane's value (its number in the workgroup) begins, and in `end` where all end. width: at most the workgroup's lanes.
+template <int kWaves>
+__device__ __forceinline__ uint32_t begins(uint32_t* s_count, uint32_t width, uint32_t begin, uint32_t& end) {
+  __shared__ uint32_t s_sum[kWaves];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  uint32_t of_wave[kWaves] = {}, total = 0;
+  if (tid < width)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) of_wave[w] = s_count[w * width + tid];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += of_wave[w];
+  uint32_t upto = total;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint32_t x = __shfl_up(upto, d);
+    if (lane >= static_cast<uint32_t>(d)) upto += x;
+  }
+  if (lane == kWave - 1) s_sum[wave] = upto;
+  __syncthreads();
+  end = begin;
+#pragma unroll
+  for (uint32_t w = 0; w < kWaves; ++w) {
+    if (w < wave) begin += s_sum[w];
+    end += s_sum[w];
+  }
+  begin += upto - total;
+  uint32_t at = begin;
+  if (tid < width)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      s_count[w * width + tid] = at;
+      at += of_wave[w];
+    }
+  __syncthreads();
+  return begin;
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSplitThreads) void embedding_split_kernel(SplitArgs a) {
+  if (static_cast<int>(blockIdx.x) >= a.tiles) {
+    write_zeros<kSplitThreads>(a.sort.zero, a.sort.zero_bytes, static_cast<int64_t>(blockIdx.x) - a.tiles, static_cast<int64_t>(gridDim.x) - a.tiles);
+    return;
+  }
+  extern __shared__ uint32_t s_count[];  // [waves][shares]
+  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const uint32_t shares = 1u << a.sort.log_shares, low = shares - 1, base = blockIdx.x * static_cast<uint32_t>(kTile);
+  uint32_t key[kSplitItems], rank[kSplitItems];
+#pragma unroll
+  for (int u = 0; u < kSplitItems; ++u) {
+    const uint32_t n = base + (wave * kSplitItems + u) * kWave + lane;
+    key[u] = n < a.sort.n ? key_of<I>(a.sort, n) : kNoToken;
+  }
+  for (uint32_t i = tid; i < kSplitWaves * shares; i += kSplitThreads) s_count[i] = 0;
+  __syncthreads();
+  uint32_t* const count = s_count + wave * shares;
+#pragma unroll
+  for (int u = 0; u < kSplitItems; ++u) rank[u] = claim(count, key[u] & low, a.sort.log_shares, key[u] != kNoToken);
+  __syncthreads();
+  uint32_t end;
+  const uint32_t begin = begins<kSplitWaves>(s_count, shares, 0u, end);
+  uint32_t* const offsets = a.offsets + static_cast<int64_t>(blockIdx.x) * (shares + 1);
+  if (tid < shares) offsets[tid] = begin;
+  if (tid == 0) offsets[shares] = end;
+#pragma unroll
+  for (int u = 0; u < kSplitItems; ++u)
+    if (key[u] != kNoToken) {
+      const uint32_t to = base + count[key[u] & low] + rank[u];
+      a.numbers[to] = key[u] >> a.sort.log_shares;
+      a.from[to] = base + (wave * kSplitItems + u) * kWave + lane;
+    }
+}
+
+__global__ __launch_bounds__(kSortThreads, 8) void embedding_place_kernel(SplitArgs a) {
+  extern __shared__ uint32_t s_count[];  // [waves][share]
+  __shared__ uint32_t s_upto[kMostTiles], s_skip[kMostTiles], s_part[2][kSortWaves];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const uint32_t mine = blockIdx.x, shares = 1u << a.sort.log_shares, share = a.sort.share;
+  // of every tile: how many of its entries are this share's, and where they begin in it (as many entries belong to lower shares)
+  uint32_t here = 0, skip = 0;
+  if (tid < static_cast<uint32_t>(a.tiles)) {
+    const uint32_t* const at = a.offsets + static_cast<int64_t>(tid) * (shares + 1) + mine;
+    skip = at[0];
+    here = at[1] - skip;
+  }
+  for (uint32_t i = tid; i < kSortWaves * share; i += kSortThreads) s_count[i] = 0;
+  uint32_t upto = here, below = skip;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint32_t x = __shfl_up(upto, d);
+    if (lane >= static_cast<uint32_t>(d)) upto += x;
+    below += __shfl_xor(below, d);
+  }
+  if (lane == kWave - 1) {
+    s_part[0][wave] = upto;
+    s_part[1][wave] = below;
+  }
+  __syncthreads();
+  uint32_t first = 0, all = 0;
+  below = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kSortWaves; ++w) {
+    if (w < wave) first += s_part[0][w];
+    all += s_part[0][w];
+    below += s_part[1][w];
+  }
+  s_upto[tid] = first + upto;
+  s_skip[tid] = tid * static_cast<uint32_t>(kTile) + skip - (first + upto - here);
+  __syncthreads();
+  // this share's entry e stands in the first tile that reaches beyond it
+  auto place_in_split = [&](uint32_t e) {
+    uint32_t lo = 0, hi = static_cast<uint32_t>(a.tiles) - 1;
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (s_upto[mid] <= e) lo = mid + 1;
+      else hi = mid;
+    }
+    return s_skip[lo] + e;
+  };
+  const uint32_t per_wave = (all + kSortThreads - 1) / kSortThreads * kWave;
+  const uint32_t begin = std::min(wave * per_wave, all), end = std::min(begin + per_wave, all);
+  uint32_t* const count = s_count + wave * share;
+  // four steps held in registers: all there are, unless one share has more than 4096 entries
+  uint32_t number[kPlaceItems], from[kPlaceItems];
+  auto read = [&](uint32_t at) {
+#pragma unroll
+    for (int u = 0; u < kPlaceItems; ++u) {
+      const uint32_t e = at + u * kWave + lane;
+      number[u] = kNoToken;
+      if (e < end) {
+        const uint32_t i = place_in_split(e);
+        number[u] = a.numbers[i];
+        from[u] = a.from[i];
+      }
+    }
+  };
+  read(begin);
+  for (uint32_t at = begin; at < end; at += kWave * kPlaceItems) {
+    if (at != begin) read(at);
+#pragma unroll
+    for (int u = 0; u < kPlaceItems; ++u)
+      if (number[u] != kNoToken) atomicAdd(&count[number[u]], 1u);
+  }
+  __syncthreads();
+  uint32_t last;
+  const uint32_t start = begins<kSortWaves>(s_count, share, below, last);
+  if (tid < share) a.sort.starts[mine * share + tid] = start;
+  if (mine == shares - 1 && tid == 0) a.sort.starts[shares * share] = last;
+  for (uint32_t at = begin; at < end; at += kWave * kPlaceItems) {
+    if (per_wave > kWave * kPlaceItems) read(at);
+#pragma unroll
+    for (int u = 0; u < kPlaceItems; ++u) {
+      const uint32_t to = claim(count, number[u], a.number_bits, number[u] != kNoToken);
+      if (number[u] != kNoToken) {
+        a.sort.keys[to] = (number[u] << a.sort.log_shares) | mine;
+        a.sort.order[to] = from[u];
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- sums
 
 constexpr int kSumWaves = 4;  // per workgroup
@@ -272,15 +476,14 @@ __device__ void zero_rows(const SumArgs& a) {
   }
   __syncthreads();
   char* const to = static_cast<char*>(a.dweight) + first * a.dim * static_cast<int64_t>(sizeof(T));
-  typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
-  const vec16 none = {0u, 0u, 0u, 0u};
+  const Vec16 none = {0u, 0u, 0u, 0u};
   const uint32_t row_bytes = static_cast<uint32_t>(a.dim) * static_cast<uint32_t>(sizeof(T));
   const uint32_t bytes = static_cast<uint32_t>(rows) * row_bytes;
   if (kBytes == 16 && a.vecs >= kWave) {  // a wave per row
     for (int r = threadIdx.x / kWave; r < rows; r += kSumWaves) {
       if (!s_empty[r]) continue;
       char* const row = to + static_cast<int64_t>(r) * row_bytes;
-      for (uint32_t v = threadIdx.x % kWave; v < static_cast<uint32_t>(a.vecs); v += kWave) __builtin_nontemporal_store(none, reinterpret_cast<vec16*>(row + v * 16u));
+      for (uint32_t v = threadIdx.x % kWave; v < static_cast<uint32_t>(a.vecs); v += kWave) __builtin_nontemporal_store(none, reinterpret_cast<Vec16*>(row + v * 16u));
     }
     return;
   }
@@ -293,7 +496,7 @@ __device__ void zero_rows(const SumArgs& a) {
     bool all = end - begin == 16u;
     for (uint32_t r = row; all && r <= last; ++r) all = s_empty[r];
     if (all) {
-      *reinterpret_cast<vec16*>(to + begin) = none;
+      *reinterpret_cast<Vec16*>(to + begin) = none;
       continue;
     }
     for (uint32_t b = begin; b < end; b += sizeof(T)) {
@@ -470,8 +673,9 @@ int log_shares_of(int64_t vocab) {
 }
 
 struct Workspace {  // of the gradient
-  int64_t keys, order, starts, partial, bytes;
-  int log_shares;
+  int64_t keys, order, starts, partial, numbers, from, offsets, bytes;
+  bool split;
+  int tiles, log_shares;
   int64_t share, pitch;
 };
 
@@ -488,6 +692,15 @@ Workspace workspace_of(int64_t n, int64_t vocab, int64_t dim) {
   w.keys = take(n * 4);
   w.order = take(n * 4);
   w.starts = take(((w.share << w.log_shares) + 1) * 4);
+  // In one launch, split: 8192 tokens 10.5 and 11.3 us (256 rows), 11.4 and 13.1 (131072 rows); 12288 tokens 16.4 and 12.1, 16.0 and 13.9; 65536
+  // tokens 67 and 29, 66 and 19. With more shares or tiles than LDS holds: one launch.
+  w.tiles = static_cast<int>((n + kTile - 1) / kTile);
+  w.split = n > kOneLaunch && n <= int64_t(kTile) * kMostTiles && w.log_shares <= 9;
+  if (w.split) {
+    w.numbers = take(n * 4);
+    w.from = take(n * 4);
+    w.offsets = take(w.tiles * ((int64_t(1) << w.log_shares) + 1) * 4);
+  }
   const int chunk = chunk_of(n, dim);
   const int64_t chunks = (n + chunk - 1) / chunk;
   w.partial = take(chunks > 1 ? chunks * 2 * w.pitch * 4 : 0);
@@ -573,17 +786,32 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     while (hidden * row_bytes % 16 != 0) --hidden;
     s.zero = dweight;
     s.zero_bytes = hidden * row_bytes;
-    const dim3 shares((1u << ws.log_shares) + static_cast<unsigned>(std::min<int64_t>((s.zero_bytes + 65535) / 65536, 1024)));
+    const unsigned shares = 1u << ws.log_shares, zeroing = static_cast<unsigned>(std::min<int64_t>((s.zero_bytes + 65535) / 65536, 1024));
     const unsigned lds = kSortWaves * s.share * 4;
-    const int held = static_cast<int>(s.per_wave / kWave);
-    auto sort = [&](auto h) {
-      if (index_dtype == TDM_I64) hipLaunchKernelGGL((embedding_sort_kernel<int64_t, h.value>), shares, dim3(kSortThreads), lds, st, s);
-      else hipLaunchKernelGGL((embedding_sort_kernel<int32_t, h.value>), shares, dim3(kSortThreads), lds, st, s);
-    };
-    if (held <= 4) sort(std::integral_constant<int, 4>{});
-    else if (held <= 8) sort(std::integral_constant<int, 8>{});
-    else sort(std::integral_constant<int, 16>{});
-    check_launch("embedding_sort launch");
+    if (ws.split) {
+      SplitArgs p{};
+      p.sort = s;
+      p.numbers = reinterpret_cast<uint32_t*>(base + ws.numbers);
+      p.from = reinterpret_cast<uint32_t*>(base + ws.from);
+      p.offsets = reinterpret_cast<uint32_t*>(base + ws.offsets);
+      p.tiles = ws.tiles;
+      while ((s.share - 1) >> p.number_bits != 0) ++p.number_bits;
+      const dim3 grid(static_cast<unsigned>(ws.tiles) + zeroing);
+      if (index_dtype == TDM_I64) hipLaunchKernelGGL((embedding_split_kernel<int64_t>), grid, dim3(kSplitThreads), kSplitWaves * shares * 4, st, p);
+      else hipLaunchKernelGGL((embedding_split_kernel<int32_t>), grid, dim3(kSplitThreads), kSplitWaves * shares * 4, st, p);
+      check_launch("embedding_split launch");
+      hipLaunchKernelGGL(embedding_place_kernel, dim3(shares), dim3(kSortThreads), lds, st, p);
+      check_launch("embedding_place launch");
+    } else {
+      const int held = static_cast<int>(s.per_wave / kWave);
+      auto sort = [&](auto h) {
+        if (index_dtype == TDM_I64) hipLaunchKernelGGL((embedding_sort_kernel<int64_t, h.value>), dim3(shares + zeroing), dim3(kSortThreads), lds, st, s);
+        else hipLaunchKernelGGL((embedding_sort_kernel<int32_t, h.value>), dim3(shares + zeroing), dim3(kSortThreads), lds, st, s);
+      };
+      if (held <= 4) sort(std::integral_constant<int, 4>{});
+      else sort(std::integral_constant<int, 8>{});
+      check_launch("embedding_sort launch");
+    }
 
     const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
     SumArgs a{};

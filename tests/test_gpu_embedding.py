@@ -157,6 +157,33 @@ def test_gradient_of_more_tokens_than_one_merge_takes():
         check_grad(ops.embedding_grad(grad.to(DEV), tokens.to(DEV), 5000), grad, tokens, 5000)
 
 
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 511, 512, 513, 32768, 32769, 131072, 262144, 262145])
+@pytest.mark.parametrize("n,kind", [(8192, "text"), (8193, "text"), (8193, "same"), (12288, "outside"), (12289, "distinct"), (20000, "same"), (41000, "text")])
+def test_every_way_of_sorting(vocab, n, kind):
+    """Both sides of the sizes where the sort takes another form: 8192 tokens, 262144 rows; whole and ragged tiles, one token for all, few tokens,
+    as many as there are. Counts and sums of small whole numbers are exact in fp32 below 2^24."""
+    from tandem_amd import ops
+
+    tokens = make_tokens(kind, n, vocab, 12)
+    g = torch.Generator().manual_seed(13)
+    grad = torch.stack([torch.ones(n), torch.arange(n) % 97.0, torch.randn(n, generator=g)], 1)
+    got = ops.embedding_grad(grad.to(DEV), tokens.to(DEV), vocab)
+    check_grad(got, grad, tokens, vocab)
+    want, _, count = exact_grad(grad, tokens, vocab, 1.0, None)
+    assert torch.equal(got[:, :2].cpu().double(), want[:, :2])  # whole numbers below 2^24
+    assert torch.equal(got, ops.embedding_grad(grad.to(DEV), tokens.to(DEV), vocab))
+
+
+def test_more_tokens_than_the_tiles_of_a_split():
+    from tandem_amd import ops
+
+    n = (1 << 22) + 4097
+    tokens = make_tokens("text", n, 3000, 14)
+    grad = torch.ones(n, 1)
+    got = ops.embedding_grad(grad.to(DEV), tokens.to(DEV), 3000)
+    assert torch.equal(got[:, 0].cpu().long(), torch.bincount(tokens, minlength=3000))
+
+
 def test_no_tokens_at_all():
     from tandem_amd import ops
 
