@@ -156,8 +156,8 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
   float* const s_val = reinterpret_cast<float*>(s_col + a.k);
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
-  const float inv_t = 1.0f / a.temperature;
-  const float c = soft ? kLog2e * inv_t : kLog2e;  // without kMix: T where a = 1, else T = 1 or a = 0
+  const float inv_t = uniform(1.0f / a.temperature);
+  const float c = uniform(soft ? kLog2e * inv_t : kLog2e);  // without kMix: T where a = 1, else T = 1 or a = 0
 
   auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
 
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
   }
   __syncthreads();
   const float counted = a.counts ? fmaxf(sum_of<kWaves>(s_part[0][lane % kWaves]), 1.0f) : a.count == nullptr ? a.divisor : *a.count;
-  const float scale = a.scale / counted;
+  const float scale = uniform(a.scale / counted);
   __syncthreads();  // s_part is the rows' from here on
 
   for (int turn = 0; row < a.rows; turn ^= 1) {
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
     const bool idle = !taught && !hard && !any_bad;  // the teacher says nothing: zeros, whatever the logits are
     // nothing but -inf: the definition has no value
     const float wrong = any_bad || (m == -__builtin_inff() && !idle) ? __builtin_nanf("") : 0.0f;
-    const float base = base_of(m);
+    const float base = uniform(base_of(m));
 
     // the loss
     float p = 0.0f;
@@ -351,8 +351,8 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
 
     // the gradient: from the sums, then the teacher's columns and the target again, with what they take off
     const float s = scale * up + wrong;
-    const float w_t = taught ? s * a.weight * a.temperature : wrong, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
-    const float k_t = (kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z), k_1 = kMix ? w_1 * __builtin_amdgcn_rcpf(z1) : 0.0f;
+    const float w_t = uniform(taught ? s * a.weight * a.temperature : wrong), w_1 = uniform(hard ? s * (1.0f - a.weight) : 0.0f);
+    const float k_t = uniform((kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z)), k_1 = kMix ? uniform(w_1 * __builtin_amdgcn_rcpf(z1)) : 0.0f;
     auto slope = [&](float f) {
       float e = k_t * exp2_of((f - base) * c);
       if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
     // 16-bit gradients: one multiply-add and the exponential, k and the row's maximum in the exponent, the sign of k apart. That is off by
     // 2^-24 of the exponent's terms: far less than the store's rounding while they stay below 1024. Other rows, and
     // what does not fit the registers, are read again.
-    const float off = __builtin_amdgcn_logf(fabsf(k_t)) - base * c, off1 = kMix ? __builtin_amdgcn_logf(fabsf(k_1)) - base * kLog2e : 0.0f;
+    const float off = uniform(__builtin_amdgcn_logf(fabsf(k_t)) - base * c), off1 = kMix ? uniform(__builtin_amdgcn_logf(fabsf(k_1)) - base * kLog2e) : 0.0f;
     const uint32_t sign = s < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
     const bool held_fits = sizeof(T) == 4 || (fabsf(base * c) < 1024.0f && (!kMix || fabsf(base * kLog2e) < 1024.0f));
     if constexpr (kHeld > 0) {

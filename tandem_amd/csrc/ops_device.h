@@ -131,6 +131,9 @@ __device__ __forceinline__ float over_wave(float x, float none, F f) {
   x = dpp_step<0x143, 0xc>(x, none, f);
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
+// A value that is the same in all lanes, in a scalar register.
+__device__ __forceinline__ float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
+
 // Over every row of 16 lanes, every lane gets it: neighbours, pairs, mirrored quads, mirrored eights.
 template <class F>
 __device__ __forceinline__ float all_16(float x, F f) {
