@@ -105,7 +105,7 @@ struct Sums {
 template <int kThreads>
 __device__ __forceinline__ float counted_by_wave(const DistillArgs& a) {
   float n = 0.0f;
-#pragma unroll 8
+#pragma unroll 16
   for (int64_t r = threadIdx.x; r < a.rows; r += kThreads) n += index_of(a.targets, a.targets_i64, r) != a.ignore ? 1.0f : 0.0f;
   return wave_sum(n);
 }
