@@ -63,10 +63,12 @@ class Attention(nn.Module):
             self._seq, self._turn = cfg.seq, {}
 
     def _rotation(self, device):
-        """(positions 0 .. seq - 1, angles per position) on `device`; not buffers, which a cast of the model would round."""
+        """(positions 0 .. seq - 1, angles per position) on `device`; not buffers, which a cast of the model would round. Kept for every later
+        call: copied from the host, so that they are there for any stream, and no inference tensors, which training could not save."""
         if device not in self._turn:
             per_head = self.q_norm.shape[0]
-            self._turn[device] = (torch.arange(self._seq, device=device), ops.rope_frequencies(per_head, device=device))
+            with torch.inference_mode(False):
+                self._turn[device] = (torch.arange(self._seq, device="cpu").to(device), ops.rope_frequencies(per_head, device=device))
         return self._turn[device]
 
     def forward(self, x):

@@ -165,7 +165,7 @@ def rope_frequencies(rotary_dim, base=10000.0, device="cuda"):
     """The rotation's angles per position: base ** (-2 i / rotary_dim) for i < rotary_dim / 2, float64."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"an even number of rotated elements, not {rotary_dim}")
-    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device="cpu")
     return (base ** (-i / rotary_dim)).to(device)
 
 

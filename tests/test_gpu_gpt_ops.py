@@ -106,6 +106,21 @@ def test_loss_and_every_gradient_against_the_model_written_out():
         assert off <= 2e-3 * grads[n].norm() + 1e-9, (n, float(off), float(grads[n].norm()))
 
 
+def test_a_first_call_in_inference_mode_leaves_training_as_it_is():
+    no_library_attention()
+    data = batch(config(), 4)
+    model, fresh = model_on_gpu(), model_on_gpu()
+    with torch.inference_mode():
+        seen = loss_of(model, *data)
+    loss = loss_of(model, *data)
+    loss.backward()
+    want = loss_of(fresh, *data)
+    want.backward()
+    assert float(seen) == float(loss.detach()) == float(want.detach())
+    for (n, p), q in zip(model.named_parameters(), fresh.parameters()):
+        assert torch.allclose(p.grad, q.grad, rtol=1e-5, atol=1e-7), n
+
+
 def test_the_plain_model_learns_from_a_teacher_too():
     from tandem_amd import ops
     from tandem_amd.model import GPT, Config
