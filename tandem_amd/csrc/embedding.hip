@@ -786,6 +786,32 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     while (hidden * row_bytes % 16 != 0) --hidden;
     s.zero = dweight;
     s.zero_bytes = hidden * row_bytes;
+    const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
+    SumArgs a{};
+    a.grad = grad;
+    a.keys = s.keys;
+    a.order = s.order;
+    a.starts = s.starts;
+    a.dweight = dweight;
+    a.partial = reinterpret_cast<float*>(base + ws.partial);
+    a.vocab = vocab;
+    a.dim = dim;
+    a.pitch = ws.pitch;
+    a.share = s.share;
+    a.log_shares = s.log_shares;
+    a.all = s.share << s.log_shares;
+    a.chunk = chunk_of(n, dim);
+    a.vecs = static_cast<int>(dim * es / width);
+    a.slices = (a.vecs + kWave - 1) / kWave;
+    a.zero_from = hidden;
+    a.zero_rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kZeroRows, kZeroBytes / row_bytes)));
+    a.scale = scale;
+    const int64_t chunks = (n + a.chunk - 1) / a.chunk;
+    const int64_t sums = (chunks * a.slices + kSumWaves - 1) / kSumWaves;
+    const int64_t zeros = (vocab - hidden + a.zero_rows - 1) / a.zero_rows;
+    require(sums + zeros < (int64_t(1) << 24), "embedding_grad: too many tokens, rows or columns for one launch");
+    a.sums = static_cast<uint32_t>(sums);
+
     const unsigned shares = 1u << ws.log_shares, zeroing = static_cast<unsigned>(std::min<int64_t>((s.zero_bytes + 65535) / 65536, 1024));
     const unsigned lds = kSortWaves * s.share * 4;
     if (ws.split) {
@@ -813,31 +839,6 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
       check_launch("embedding_sort launch");
     }
 
-    const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
-    SumArgs a{};
-    a.grad = grad;
-    a.keys = s.keys;
-    a.order = s.order;
-    a.starts = s.starts;
-    a.dweight = dweight;
-    a.partial = reinterpret_cast<float*>(base + ws.partial);
-    a.vocab = vocab;
-    a.dim = dim;
-    a.pitch = ws.pitch;
-    a.share = s.share;
-    a.log_shares = s.log_shares;
-    a.all = s.share << s.log_shares;
-    a.chunk = chunk_of(n, dim);
-    a.vecs = static_cast<int>(dim * es / width);
-    a.slices = (a.vecs + kWave - 1) / kWave;
-    a.zero_from = hidden;
-    a.zero_rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kZeroRows, kZeroBytes / row_bytes)));
-    a.scale = scale;
-    const int64_t chunks = (n + a.chunk - 1) / a.chunk;
-    const int64_t sums = (chunks * a.slices + kSumWaves - 1) / kSumWaves;
-    const int64_t zeros = (vocab - hidden + a.zero_rows - 1) / a.zero_rows;
-    require(sums + zeros < (int64_t(1) << 24), "embedding_grad: too many tokens, rows or columns for one launch");
-    a.sums = static_cast<uint32_t>(sums);
     if (sums + zeros == 0) return;
     with_dtype(dtype, [&](auto t) {
       using T = decltype(t);

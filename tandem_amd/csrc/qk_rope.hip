@@ -551,9 +551,9 @@ int tdm_k6_qk_norm_rope(const tdm_qk_shape* shape, const tdm_heads* q, const tdm
       using T = decltype(t);
       with_run(p.run, [&](auto v, auto c) {
         if constexpr (v.value * sizeof(T) <= 16) {
-            if (p.args.interleaved) hipLaunchKernelGGL((qk_rope_kernel<T, v.value, c.value, true>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.args);
-            else hipLaunchKernelGGL((qk_rope_kernel<T, v.value, c.value, false>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.args);
-          }
+          if (p.args.interleaved) hipLaunchKernelGGL((qk_rope_kernel<T, v.value, c.value, true>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.args);
+          else hipLaunchKernelGGL((qk_rope_kernel<T, v.value, c.value, false>), grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), p.args);
+        }
       });
     });
     check_launch("qk_rope launch");
@@ -613,8 +613,7 @@ int tdm_k6_qk_norm_rope_grad(const tdm_qk_shape* shape, const tdm_heads* dq_out,
       using T = decltype(t);
       if (groups > 0) {
         with_run(p.run, [&](auto v, auto c) {
-          if constexpr (v.value * sizeof(T) <= 16)
-  {
+          if constexpr (v.value * sizeof(T) <= 16) {
             if (p.args.interleaved) hipLaunchKernelGGL((qk_rope_grad_kernel<T, v.value, c.value, true>), dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, st, p.args);
             else hipLaunchKernelGGL((qk_rope_grad_kernel<T, v.value, c.value, false>), dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, st, p.args);
           }

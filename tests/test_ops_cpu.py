@@ -59,6 +59,8 @@ def test_embedding_argument_errors_need_no_gpu():
     refused(grad(p, p, i64, p, ctypes.c_void_p(4100), need, 10_000, 4, 4, f32, 1.0, -1), "16 bytes")
     refused(grad(p, p, i64, None, p, need, 10_000, 4, 4, f32, 1.0, -1), "null")
     refused(grad(p, p, 7, p, p, need, 10_000, 4, 4, f32, 1.0, -1), "int64")
+    most, wide = 1 << 28, 1 << 20  # refused before the first launch, which would write
+    refused(grad(p, p, i64, p, p, L.tdm_k5_embedding_grad_workspace(most, 4, wide), most, 4, wide, f32, 1.0, -1), "one launch")
 
 
 def test_qk_norm_rope_refuses_cpu_tensors_and_odd_rotations():
@@ -152,3 +154,15 @@ def test_the_rotary_model_s_parameters_and_refusals():
     plain = GPT(Config(seq=16, layers=1, heads=2, dim=16))
     with pytest.raises(ValueError, match="no CPU path"):
         plain(torch.zeros(1, 4, dtype=torch.int64), teacher=(torch.zeros(1, 4, 2, dtype=torch.int64), torch.zeros(1, 4, 2)))
+
+
+def test_the_rotary_model_keeps_no_inference_tensors():
+    """What a first call without gradients leaves behind has to serve a training step; tensors of inference mode cannot be saved for one."""
+    from tandem_amd.model import GPT, Config
+
+    attention = GPT(Config(seq=16, layers=1, heads=2, dim=16, rotary=True)).blocks[0].attn
+    with torch.inference_mode():
+        first = attention._rotation(torch.device("cpu"))
+    assert not any(t.is_inference() for t in first)
+    assert first[0].tolist() == list(range(16)) and first[1].dtype == torch.float64
+    assert attention._rotation(torch.device("cpu")) is first
