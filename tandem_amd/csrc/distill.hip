@@ -71,7 +71,34 @@ __device__ __forceinline__ Body body_of(const T* x, int64_t vocab) {
 // lowest value.
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
-template <bool kMix>
+// What the two temperatures, T and 1, need of d = x - m: kOne exponential where one of them does for both parts (a = 0, a = 1 or T = 1);
+// kTwo; or one again, F, of which both are powers, for the usual T = 2 (F, F^2) and T = 1.5 (F^2, F^3): 1031 rows of 50021 fp16
+// logits take 56 us instead of 64, 4096 rows 196 and 201 instead of 212.
+enum Mix { kOne, kTwo, kSquare, kCube };
+Mix mix_of(float weight, float temperature) {
+  if (weight <= 0.0f || weight >= 1.0f || temperature == 1.0f) return kOne;
+  return temperature == 2.0f ? kSquare : temperature == 1.5f ? kCube : kTwo;
+}
+// What d is multiplied with in F's exponent: log2(e) / T, of kCube log2(e) / 3.
+template <Mix kMix>
+__device__ __forceinline__ float rate_of(const DistillArgs& a) {
+  return kMix == kCube ? kLog2e / 3.0f : a.weight > 0.0f ? kLog2e / a.temperature : kLog2e;
+}
+template <Mix kMix>
+struct Powers {  // soft = exp(d / T), hard = exp(d)
+  float f, other = 0.0f;
+  __device__ __forceinline__ Powers(float d, float c) : f(exp2_of(d * c)) {
+    if (kMix == kTwo) other = exp2_of(d * kLog2e);
+  }
+  __device__ __forceinline__ float soft() const { return kMix == kCube ? f * f : f; }
+  __device__ __forceinline__ float hard() const { return kMix == kOne ? f : kMix == kTwo ? other : soft() * f; }
+  __device__ __forceinline__ float add_hard(float to) const { return kMix == kOne ? 0.0f : kMix == kTwo ? to + other : fmaf(soft(), f, to); }
+  __device__ __forceinline__ float weighed(float of_soft, float of_hard) const {
+    return kMix == kOne ? of_soft * f : kMix == kTwo ? fmaf(of_hard, other, of_soft * f) : soft() * fmaf(of_hard, f, of_soft);
+  }
+};
+
+template <Mix kMix>
 struct Sums {
   float m = -__builtin_inff(), z = 0.0f, z1 = 0.0f;
 
@@ -85,18 +112,21 @@ struct Sums {
     float s = 0.0f, s1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      s += exp2_of((f[i] - base) * c);
-      if (kMix) s1 += exp2_of((f[i] - base) * kLog2e);
+      const Powers<kMix> e(f[i] - base, c);
+      s += e.soft();
+      s1 = e.add_hard(s1);
     }
-    z = fmaf(z, exp2_of((m - base) * c), s);
-    if (kMix) z1 = fmaf(z1, exp2_of((m - base) * kLog2e), s1);
+    const Powers<kMix> e(m - base, c);
+    z = fmaf(z, e.soft(), s);
+    if (kMix != kOne) z1 = fmaf(z1, e.hard(), s1);
     m = top;
   }
   // the same sums with the maximum `top` of several
   __device__ __forceinline__ void lift(float top, float c) {
     const float base = base_of(top);
-    z *= exp2_of((m - base) * c);
-    if (kMix) z1 *= exp2_of((m - base) * kLog2e);
+    const Powers<kMix> e(m - base, c);
+    z *= e.soft();
+    if (kMix != kOne) z1 *= e.hard();
     m = top;
   }
 };
@@ -144,8 +174,7 @@ constexpr uint32_t kNoColumn = 0xffffffffu;
 // its vectors makes room for the next row's: loads, exponentials and stores are under way at the same time with one workgroup per
 // compute unit. The teacher's entries are one lane's each (k <= kG): their elements and the target's are written again after the row, behind
 // a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries.
-// kMix: both temperatures are needed (0 < a < 1 and T != 1); otherwise one exponential does for both parts.
-template <typename T, int kG, int kHeld, bool kMix>
+template <typename T, int kG, int kHeld, Mix kMix>
 __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(DistillArgs a, int log_table) {
   constexpr int kN = per_vec<T>(), kWaves = kG / kWave;
   __shared__ WaveRow s_wave[2][kWaves];
@@ -157,7 +186,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
   const float inv_t = uniform(1.0f / a.temperature);
-  const float c = uniform(soft ? kLog2e * inv_t : kLog2e);  // without kMix: T where a = 1, else T = 1 or a = 0
+  const float c = uniform(rate_of<kMix>(a));
 
   auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
 
@@ -300,7 +329,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
     mine.m = wave_max(sums.m);
     sums.lift(mine.m, c);
     mine.z = wave_sum(sums.z);
-    mine.z1 = kMix ? wave_sum(sums.z1) : mine.z;
+    mine.z1 = kMix != kOne ? wave_sum(sums.z1) : mine.z;
     float m = mine.m, z = mine.z, z1 = mine.z1, t_m = mine.t_m, t_z = mine.t_z;
     bool any_twice = mine.flags & kTwice, any_bad = mine.flags & kBad;
     if constexpr (kWaves > 1) {
@@ -314,7 +343,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
       part.z1 = w.z1;
       part.lift(m, c);
       z = sum_of<kWaves>(part.z);
-      z1 = kMix ? sum_of<kWaves>(part.z1) : z;
+      z1 = kMix != kOne ? sum_of<kWaves>(part.z1) : z;
       if (soft) {
         t_m = max_of<kWaves>(w.t_m);
         t_z = sum_of<kWaves>(w.t_z * exp2_of((w.t_m - base_of(t_m)) * ck));
@@ -352,22 +381,22 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
     // the gradient: from the sums, then the teacher's columns and the target again, with what they take off
     const float s = scale * up + wrong;
     const float w_t = uniform(taught ? s * a.weight * a.temperature : wrong), w_1 = uniform(hard ? s * (1.0f - a.weight) : 0.0f);
-    const float k_t = uniform((kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z)), k_1 = kMix ? uniform(w_1 * __builtin_amdgcn_rcpf(z1)) : 0.0f;
+    const float k_t = uniform((kMix != kOne ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z)), k_1 = kMix != kOne ? uniform(w_1 * __builtin_amdgcn_rcpf(z1)) : 0.0f;
     auto slope = [&](float f) {
-      float e = k_t * exp2_of((f - base) * c);
-      if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
-      return e;
+      return Powers<kMix>(f - base, c).weighed(k_t, k_1);
     };
     if (g != nullptr && edge >= 0) g[edge] = narrow<T>(idle ? 0.0f : slope(edge_x) + wrong);
     if (g != nullptr && idle) write_zeros(g);
     const uint32_t my_col = col;
     if (next < a.rows) fetch_small(next, nx, next_body);
-    // 16-bit gradients: one multiply-add and the exponential, k and the row's maximum in the exponent, the sign of k apart. That is off by
-    // 2^-24 of the exponent's terms: far less than the store's rounding while they stay below 1024. Other rows, and
-    // what does not fit the registers, are read again.
-    const float off = uniform(__builtin_amdgcn_logf(fabsf(k_t)) - base * c), off1 = kMix ? uniform(__builtin_amdgcn_logf(fabsf(k_1)) - base * kLog2e) : 0.0f;
-    const uint32_t sign = s < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
-    const bool held_fits = sizeof(T) == 4 || (fabsf(base * c) < 1024.0f && (!kMix || fabsf(base * kLog2e) < 1024.0f));
+    // 16-bit gradients: one multiply-add and the exponential, the row's maximum in the exponent, and where every exponential has a factor of its
+    // own that too, its sign apart. That is off by 2^-24 of the exponent's terms: far less than the store's rounding while they
+    // stay below 1024. Other rows, and what does not fit the registers, are read again.
+    constexpr bool kApart = kMix == kOne || kMix == kTwo;
+    const float off = uniform((kApart ? __builtin_amdgcn_logf(fabsf(k_t)) : 0.0f) - base * c);
+    const float off1 = kMix == kTwo ? uniform(__builtin_amdgcn_logf(fabsf(k_1)) - base * kLog2e) : 0.0f;
+    const uint32_t sign = kApart && s < 0.0f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+    const bool held_fits = sizeof(T) == 4 || (fabsf(base * c) < 1024.0f && (kMix != kTwo || fabsf(base * kLog2e) < 1024.0f));
     if constexpr (kHeld > 0) {
       from = stretch(nx + next_body.head, next < a.rows ? next_body.vecs * 16 : 0);
       const __amdgpu_buffer_rsrc_t to = stretch(g + body.head, g != nullptr && !idle && held_fits ? body.vecs * 16 : 0);
@@ -380,10 +409,14 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
 #pragma unroll
           for (int e = 0; e < kN; ++e) {
             if constexpr (sizeof(T) == 4) f[e] = slope(f[e]);
-            else f[e] = exp2_of(fmaf(f[e], c, off)) + (kMix ? exp2_of(fmaf(f[e], kLog2e, off1)) : 0.0f);
+            else if constexpr (kApart) f[e] = exp2_of(fmaf(f[e], c, off)) + (kMix == kTwo ? exp2_of(fmaf(f[e], kLog2e, off1)) : 0.0f);
+            else {
+              const float p = exp2_of(fmaf(f[e], c, off));
+              f[e] = (kMix == kCube ? p * p : p) * fmaf(k_1, p, k_t);
+            }
           }
           Vec16 out = pack16<T>(f);
-          if constexpr (sizeof(T) == 2) out ^= sign;
+          if constexpr (sizeof(T) == 2 && kApart) out ^= sign;
           store16<kStream>(out, to, lane16, i * kG * 16);
         }
         if (i < kEarly) held[i] = load16<kStream>(from, lane16, i * kG * 16);
@@ -432,7 +465,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
 // floats, 16 entries, two temperatures: 14.1 us with a wave a row). kHeld vectors of the row and kEntries of the teacher's entries per lane.
 constexpr int kShortLanes = 16, kShortThreads = 256, kShortRows = kShortThreads / kShortLanes;
 
-template <typename T, int kHeld, int kEntries, bool kMix>
+template <typename T, int kHeld, int kEntries, Mix kMix>
 __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArgs a) {
   constexpr int kN = per_vec<T>();
   extern __shared__ uint32_t s_short[];  // k columns and k values of every row
@@ -441,7 +474,7 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
   uint32_t* const s_col = s_short + place * 2 * a.k;
   float* const s_val = reinterpret_cast<float*>(s_col + a.k);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
-  const float inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = soft ? ck : kLog2e;
+  const float inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = rate_of<kMix>(a);
   const float lowest = -__builtin_inff();
 
   const int64_t asked = static_cast<int64_t>(blockIdx.x) * kShortRows + place, row = std::min(asked, a.rows - 1);
@@ -504,7 +537,7 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
   }
   const float m = all_16(sums.m, Max{}), base = base_of(m);
   sums.lift(m, c);
-  const float z = all_16(sums.z, Add{}), z1 = kMix ? all_16(sums.z1, Add{}) : z;
+  const float z = all_16(sums.z, Add{}), z1 = kMix != kOne ? all_16(sums.z1, Add{}) : z;
   const float t_m = all_16(t_top, Max{});
   float t_sum = 0.0f;
 #pragma unroll
@@ -548,12 +581,10 @@ __global__ __launch_bounds__(kShortThreads) void distill_short_kernel(DistillArg
   }
   const float s = a.scale / count * up + wrong;
   const float w_t = taught ? s * a.weight * a.temperature : wrong, w_1 = hard ? s * (1.0f - a.weight) : 0.0f;
-  const float k_t = (kMix ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z), k_1 = kMix ? w_1 * __builtin_amdgcn_rcpf(z1) : 0.0f;
+  const float k_t = (kMix != kOne ? w_t : w_t + w_1) * __builtin_amdgcn_rcpf(z), k_1 = kMix != kOne ? w_1 * __builtin_amdgcn_rcpf(z1) : 0.0f;
   const bool zeros = !counted || idle;
   auto slope = [&](float f) {
-    float e = k_t * exp2_of((f - base) * c);
-    if (kMix) e = fmaf(k_1, exp2_of((f - base) * kLog2e), e);
-    return e;
+    return Powers<kMix>(f - base, c).weighed(k_t, k_1);
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
@@ -612,7 +643,7 @@ __global__ __launch_bounds__(kFoldThreads) void distill_sum_kernel(DistillArgs a
 // per row, with the teacher's share.
 constexpr int kSliceThreads = 256, kMostSlices = kWave;
 
-template <typename T, bool kMix>
+template <typename T, Mix kMix>
 __global__ __launch_bounds__(kSliceThreads) void distill_slice_kernel(DistillArgs a, int slices, int per_slice, WaveRow* parts) {
   constexpr int kN = per_vec<T>(), kWaves = kSliceThreads / kWave, kAhead = 4;
   __shared__ WaveRow s_wave[kWaves];
@@ -621,7 +652,7 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slice_kernel(DistillArg
   if (a.targets != nullptr && index_of(a.targets, a.targets_i64, row) == a.ignore) return;
   const T* const x = static_cast<const T*>(a.logits) + row * a.vocab;
   const Body body = body_of(x, a.vocab);
-  const float c = a.weight > 0.0f ? kLog2e / a.temperature : kLog2e;
+  const float c = rate_of<kMix>(a);
   Sums<kMix> sums;
   if (slice == 0) {
     const int edge = tid < body.head ? tid : tid - body.head < body.tail ? body.head + body.vecs * kN + tid - body.head : -1;
@@ -647,7 +678,7 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slice_kernel(DistillArg
   mine.m = wave_max(sums.m);
   sums.lift(mine.m, c);
   mine.z = wave_sum(sums.z);
-  mine.z1 = kMix ? wave_sum(sums.z1) : mine.z;
+  mine.z1 = kMix != kOne ? wave_sum(sums.z1) : mine.z;
   if (tid % kWave == 0) s_wave[tid / kWave] = mine;
   __syncthreads();
   if (tid >= kWave) return;
@@ -660,15 +691,15 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slice_kernel(DistillArg
   all.m = max_of<kWaves>(w.m);
   part.lift(all.m, c);
   all.z = sum_of<kWaves>(part.z);
-  all.z1 = kMix ? sum_of<kWaves>(part.z1) : all.z;
+  all.z1 = kMix != kOne ? sum_of<kWaves>(part.z1) : all.z;
   if (tid == 0) parts[blockIdx.x] = all;
 }
 
-template <typename T, bool kMix>
+template <typename T, Mix kMix>
 __global__ __launch_bounds__(kFoldThreads) void distill_slices_loss_kernel(DistillArgs a, int slices, const WaveRow* parts, float* loss, int each_row) {
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const bool soft = a.weight > 0.0f, hard = a.weight < 1.0f;
-  const float lowest = -__builtin_inff(), inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = soft ? ck : kLog2e;
+  const float lowest = -__builtin_inff(), inv_t = 1.0f / a.temperature, ck = kLog2e * inv_t, c = rate_of<kMix>(a);
   float total = 0.0f, count = 0.0f;
   for (int64_t row = wave; row < a.rows; row += kFoldThreads / kWave) {
     const int64_t y = a.targets == nullptr ? 0 : index_of(a.targets, a.targets_i64, row);
@@ -686,7 +717,7 @@ __global__ __launch_bounds__(kFoldThreads) void distill_slices_loss_kernel(Disti
     part.z1 = w.z1;
     const float m = wave_max(w.m), base = base_of(m);
     part.lift(m, c);
-    const float z = wave_sum(part.z), z1 = kMix ? wave_sum(part.z1) : z;
+    const float z = wave_sum(part.z), z1 = kMix != kOne ? wave_sum(part.z1) : z;
     bool bad = hard && (y < 0 || y >= a.vocab);
     auto entry = [&](int e, float& t) {  // its column, or -1
       const int64_t j = index_of(a.index, a.index_i64, row * a.k + e);
@@ -739,6 +770,16 @@ void check_how(const tdm_distill_how* h) {
   require(h->temperature > 0.0f && h->temperature < std::numeric_limits<float>::infinity(), "distill: the temperature must be positive and finite");
   require(h->weight >= 0.0f && h->weight <= 1.0f, "distill: the teacher's weight must lie between 0 and 1");
   require(h->reduction == TDM_DISTILL_NONE || h->reduction == TDM_DISTILL_MEAN || h->reduction == TDM_DISTILL_SUM, "distill: unknown reduction");
+}
+
+template <class F>
+void with_mix(Mix mix, F&& f) {
+  switch (mix) {
+    case kOne: f(std::integral_constant<Mix, kOne>{}); return;
+    case kSquare: f(std::integral_constant<Mix, kSquare>{}); return;
+    case kCube: f(std::integral_constant<Mix, kCube>{}); return;
+    default: f(std::integral_constant<Mix, kTwo>{}); return;
+  }
 }
 
 constexpr int64_t kCountBytes = 256;
@@ -823,8 +864,7 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
           hipLaunchKernelGGL((distill_slices_loss_kernel<T, m.value>), dim3(1), dim3(kFoldThreads), 0, st, a, slices, parts, loss, h.reduction == TDM_DISTILL_NONE);
           check_launch("distill_slices_loss launch");
         };
-        if (h.weight > 0.0f && h.weight < 1.0f && h.temperature != 1.0f) launch(std::true_type{});
-        else launch(std::false_type{});
+        with_mix(mix_of(h.weight, h.temperature), launch);
       });
       return;
     }
@@ -835,7 +875,6 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
       a.count = count;
     }
     if (h.rows > 0) {
-      const bool mix = h.weight > 0.0f && h.weight < 1.0f && h.temperature != 1.0f;
       int log_table = 6;  // at most half full
       while ((1 << log_table) < 2 * h.k) ++log_table;
       const unsigned lds = ((1u << log_table) + 2u * h.k) * 4u;
@@ -869,8 +908,7 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
           else if (vecs <= 16384) launch(g1024, integral_constant<int, 16>{}, m);
           else launch(g1024, integral_constant<int, 0>{}, m);
         };
-        if (mix) pick(std::true_type{});
-        else pick(std::false_type{});
+        with_mix(mix_of(h.weight, h.temperature), pick);
       });
       check_launch("distill launch");
     }

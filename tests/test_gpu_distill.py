@@ -138,6 +138,19 @@ def test_loss_and_gradient(rows, vocab, k, dtype, index, teacher, tau, weight):
     check(x, idx, t, y if weight < 1 else None, tau, weight, scale=1024.0 if dtype == "fp16" else 1.0)
 
 
+@pytest.mark.parametrize("tau", [0.75, 1.5, 1.7, 2.0])
+@pytest.mark.parametrize("rows,vocab,k,dtype,index,teacher", [s for s in SIZES if s[1] > 2])
+def test_two_temperatures_and_a_negative_scale(rows, vocab, k, dtype, index, teacher, tau):
+    """Temperatures whose exponentials are powers of one, and others. A third power is off by three times 2 r / 3 + 2 (the hardware's
+    exponential) and its two products, (2 r + 8) u: 4 u more than counted above, of the 40 u that sums have beyond V / 64, 20 of
+    which no sum here needs (6 steps over lanes, 4 over waves, a vector's 8 and a step of the maximum's)."""
+    x, idx, t, y = make(rows, vocab, k, dtype, 11, index, teacher, ignored=0.2)
+    check(x, idx, t, y, tau, 0.4, "sum", scale=-64.0)
+    x[0, vocab // 2] = 4000.0  # the exponent's terms are too large to be added up beforehand
+    x[0, 0] = -INF
+    check(x, idx, t, y, tau, 0.4, "none", scale=-64.0)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 31, 32, 33])
 def test_the_loss_alone_of_a_few_long_rows(rows):
     for vocab, dtype, k in ((20001, "fp32", 70), (131072, "bf16", 64), (33000, "fp16", 1000)):
