@@ -175,7 +175,7 @@ constexpr uint32_t kNoColumn = 0xffffffffu;
 // compute unit. The teacher's entries are one lane's each (k <= kG): their elements and the target's are written again after the row, behind
 // a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries.
 template <typename T, int kG, int kHeld, Mix kMix>
-__global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(DistillArgs a, int log_table) {
+__global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_table) {
   constexpr int kN = per_vec<T>(), kWaves = kG / kWave;
   __shared__ WaveRow s_wave[2][kWaves];
   __shared__ float s_part[2][kWaves];
@@ -190,6 +190,7 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
 
   auto row_at = [&](int64_t row) { return static_cast<const T*>(a.logits) + row * a.vocab; };
 
+  constexpr int kAhead = 4;          // vectors in flight of a row that is read twice, or for its loss alone
   constexpr int kEarly = kHeld / 2;  // vectors of the next row that are read while this row's gradient is written
   Vec16 held[kHeld > 0 ? kHeld : 1];
   __amdgpu_buffer_rsrc_t from = stretch(nullptr, 0);
@@ -287,10 +288,19 @@ __global__ __launch_bounds__(kG, kHeld > 16 ? 2 : 4) void distill_kernel(Distill
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      for (int v = tid; v < body.vecs; v += kG) {
-        float f[kN];
-        unpack16<T>(reinterpret_cast<const Vec16*>(x + body.head)[v], f);
-        sums.take(f, c);
+      const Vec16* const vecs = reinterpret_cast<const Vec16*>(x + body.head);
+      for (int v = tid; v < body.vecs; v += kG * kAhead) {
+        Vec16 ahead[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (v + u * kG < body.vecs) ahead[u] = vecs[v + u * kG];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (v + u * kG < body.vecs) {
+            float f[kN];
+            unpack16<T>(ahead[u], f);
+            sums.take(f, c);
+          }
       }
     }
     {
@@ -868,7 +878,12 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
       });
       return;
     }
-    if (a.counts && (h.rows > kCountRows || (h.k <= 64 && all_vecs > 64 && all_vecs <= 256))) {  // a workgroup of one wave does not count
+    // One wave per row where that suffices: what a row needs once (a chain of loads, sums over lanes, logarithms) takes a larger workgroup as
+    // long, and fewer rows are under way then. 16384 rows of 3500 fp16 logits: 65 us with one wave, 127 with four; of
+    // 8000 logits 2048 rows 20 and 24 us, but 1024 rows 14.5 and 14.4, 512 rows 13.0 and 10.8.
+    const bool many = h.rows > 4 * kComputeUnits;
+    const bool one_wave = h.k <= 64 && all_vecs > 64 && (all_vecs <= 256 || (many && all_vecs <= (grad == nullptr ? 8192 : 1024)));
+    if (a.counts && (h.rows > kCountRows || one_wave)) {  // a workgroup of one wave does not count
       hipLaunchKernelGGL(distill_count_kernel, dim3(1), dim3(kFoldThreads), 0, st, a, count);
       check_launch("distill_count launch");
       a.counts = 0;
@@ -882,13 +897,14 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
         using T = decltype(t);
         const int64_t vecs = h.vocab * static_cast<int64_t>(sizeof(T)) / 16;
         auto launch = [&](auto g, auto held, auto m) {
-          // as many workgroups as the GPU holds at once: they go on to further rows
-          const int64_t grid = std::min<int64_t>(h.rows, kComputeUnits * (held.value == 0 ? 2 : g.value == 64 ? 32 : (held.value > 16 ? 512 : 1024) / g.value));
+          // about as many workgroups as the GPU holds at once: they go on to further rows
+          const int64_t grid = std::min<int64_t>(h.rows, kComputeUnits * (held.value == 0 || g.value == 64 ? 2048 : 1024) / g.value);
           hipLaunchKernelGGL((distill_kernel<T, g.value, held.value, m.value>), dim3(static_cast<unsigned>(grid)), dim3(g.value), lds, st, a, log_table);
         };
         auto pick = [&](auto m) {
           using std::integral_constant;
           const integral_constant<int, 64> g64{};
+          const integral_constant<int, 128> g128{};
           const integral_constant<int, 256> g256{};
           const integral_constant<int, 512> g512{};
           const integral_constant<int, 1024> g1024{};
@@ -900,8 +916,14 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
           if (h.k <= 16 && vecs <= 32) launch_short(integral_constant<int, 2>{}, integral_constant<int, 1>{});
           else if (h.k <= 16 && vecs <= 64) launch_short(integral_constant<int, 4>{}, integral_constant<int, 1>{});
           else if (h.k <= 64 && vecs <= 64) launch_short(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-          else if (h.k <= 64 && vecs <= 256) launch(g64, integral_constant<int, 4>{}, m);
+          else if (one_wave && vecs <= 256) launch(g64, integral_constant<int, 4>{}, m);
+          else if (one_wave && vecs <= 512) launch(g64, integral_constant<int, 8>{}, m);
+          else if (one_wave && vecs <= 1024) launch(g64, integral_constant<int, 16>{}, m);
+          else if (one_wave) launch(g64, integral_constant<int, 0>{}, m);
+          // the loss alone of long rows: nothing to keep, and more rows under way (8192 rows of 131072 fp16 logits: 399 us, held 511)
+          else if (h.k <= 256 && grad == nullptr && h.rows >= kComputeUnits) launch(g256, integral_constant<int, 0>{}, m);
           else if (h.k <= 256 && vecs <= 1024) launch(g256, integral_constant<int, 4>{}, m);
+          else if (h.k <= 128 && vecs <= 2048 && many) launch(g128, integral_constant<int, 16>{}, m);  // 4134 rows of 8970 fp16 logits: 45 us, with g256 52
           else if (h.k <= 256 && vecs <= 2048) launch(g256, integral_constant<int, 8>{}, m);
           else if (h.k <= 256 && vecs <= 4096) launch(g256, integral_constant<int, 16>{}, m);
           else if (h.k <= 512 && vecs <= 8192) launch(g512, integral_constant<int, 16>{}, m);

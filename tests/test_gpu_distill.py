@@ -151,6 +151,20 @@ def test_two_temperatures_and_a_negative_scale(rows, vocab, k, dtype, index, tea
     check(x, idx, t, y, tau, 0.4, "none", scale=-64.0)
 
 
+@pytest.mark.parametrize("rows,vocab,k,dtype", [(1024, 1500, 64, "fp32"), (1025, 1500, 64, "fp32"), (1025, 2049, 33, "fp32"), (1500, 5003, 9, "bf16"),
+                                                (1025, 9001, 64, "fp16"), (1025, 9001, 65, "bf16"), (1025, 8193, 129, "fp16"), (256, 20011, 256, "bf16"),
+                                                (255, 20011, 20, "bf16"), (260, 66003, 12, "fp16")])
+def test_many_rows_and_rows_of_few_lanes(rows, vocab, k, dtype):
+    """The sizes at which another number of lanes takes a row; loss alone, and with the gradient; a column named twice, and rows that
+    have one entry or none."""
+    x, idx, t, y = make(rows, vocab, k, dtype, 19, ignored=0.1)
+    idx[5, 1] = idx[5, 0]
+    idx[rows - 1, 1:] = -1
+    idx[7] = -1
+    check(x, idx, t, y, 2.0, 0.5, "mean", scale=256.0)
+    check(x, idx, t, None, 1.0, 1.0, "none")
+
+
 @pytest.mark.parametrize("rows", [1, 2, 31, 32, 33])
 def test_the_loss_alone_of_a_few_long_rows(rows):
     for vocab, dtype, k in ((20001, "fp32", 70), (131072, "bf16", 64), (33000, "fp16", 1000)):
