@@ -426,9 +426,10 @@ def distill_loss(logits, teacher_index, teacher_logits, targets=None, temperatur
     entries. A column, or a target that is used, outside the vocabulary and a NaN among the teacher's logits show: the row's loss
     and gradient are NaN.
 
-    logits contiguous, float32, float16 or bfloat16; the teacher's logits any of these; k at most 1024. Where a gradient is needed
-    it is computed with the loss, from one reading of the logits, and kept until the backward pass hands it out. An upstream
-    gradient other than one (a loss that is scaled or divided afterwards) makes the backward pass compute it again."""
+    logits contiguous, float32, float16 or bfloat16; the teacher's logits any of these, they take no gradient; k at most 1024. Where
+    the gradient of float32 or bfloat16 logits is needed it is computed with the loss, from one reading of the logits, and kept until
+    the backward pass hands it out; an upstream gradient other than one (a loss that is scaled or divided afterwards) makes the
+    backward pass compute it again. Of float16 logits, whose loss is scaled as a rule, the backward pass computes it."""
     how, operands = _check_distill(logits, teacher_index, teacher_logits, targets, temperature, weight, ignore_index, reduction, 1.0)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Distill.apply(logits, *operands, how, reduction == "none")
@@ -494,7 +495,9 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, targets, how, each_row):
         ctx.save_for_backward(logits, index, teacher, targets)
-        ctx.how, ctx.each_row, ctx.grad = how, each_row, _empty_at_phase_of(logits)
+        ctx.how, ctx.each_row = how, each_row
+        # float16 is trained with a scaled loss: a gradient computed here would be for nothing
+        ctx.grad = None if logits.dtype == torch.float16 else _empty_at_phase_of(logits)
         return _distill(logits, index, teacher, targets, how, each_row, True, ctx.grad, None, False)
 
     @staticmethod
