@@ -133,14 +133,20 @@ def _embedding_grad(grad, tokens, vocab, scale, padding):
     _same_device(grad, tokens)
     if grad.dim() < 1 or grad.shape[:-1] != tokens.shape or grad.shape[-1] == 0:
         raise ValueError(f"embedding_grad: a gradient of {list(grad.shape)} for tokens of {list(tokens.shape)}")
-    n, dim = tokens.numel(), grad.shape[-1]
+    need = lib().tdm_k5_embedding_grad_workspace(tokens.numel(), vocab, grad.shape[-1])
+    return _embedding_backward(grad, tokens, vocab, grad.shape[-1], scale, padding, need)
+
+
+def _embedding_backward(grad, tokens, vocab, dim, scale, padding, need):
     out = grad.new_empty((vocab, dim))
-    L = lib()
-    need = L.tdm_k5_embedding_grad_workspace(n, vocab, dim)
     work = _workspace(need, grad)
-    _call(grad, L.tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), work.data_ptr(), need, n, vocab, dim,
-          CODES[grad.dtype], scale, padding)
+    _call(grad, lib().tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), work.data_ptr(), need,
+          tokens.numel(), vocab, dim, CODES[grad.dtype], scale, padding)
     return out
+
+
+# A backward pass runs on a thread of autograd's, where Python is slow to start: what the forward pass knows is kept for it, and what
+# autograd sees to (an upstream gradient's shape, dtype and device) is not checked again.
 
 
 class _Embedding(torch.autograd.Function):
@@ -148,14 +154,15 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, tokens, weight, scale, padding):
         tokens = _indices(tokens, "embedding(tokens)")
         ctx.save_for_backward(tokens)
-        ctx.how = weight.shape[0], scale, padding
+        vocab, dim = weight.shape
+        ctx.how = vocab, dim, scale, padding, lib().tdm_k5_embedding_grad_workspace(tokens.numel(), vocab, dim)
         return _embedding(tokens, weight, scale)
 
     @staticmethod
     @_once
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
-        return None, _embedding_grad(grad.contiguous(), tokens, *ctx.how), None, None
+        return None, _embedding_backward(grad if grad.is_contiguous() else grad.contiguous(), tokens, *ctx.how), None, None
 
 
 # ---- norms of queries and keys, with the rotation
@@ -191,7 +198,8 @@ def qk_norm_rope_grad(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_f
     weight that is None has none. The weights' gradients are summed in fp32 over all tokens and heads in a fixed order."""
     x = _separate(q, k)
     how = _check_qk(x, q, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    return _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how)
+    _check_upstream(q, x, dq_out, dk_out)
+    return _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how, _qk_need(how))
 
 
 def qkv_norm_rope(qkv, q_heads, kv_heads, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False):
@@ -209,13 +217,20 @@ def qkv_norm_rope_grad(dq_out, dk_out, dv_out, qkv, q_heads, kv_heads, q_weight,
     """The gradients (dqkv, dq_weight, dk_weight) of qkv_norm_rope for the upstream gradients dq_out, dk_out, dv_out (None: zeros)."""
     x = _packed(qkv, q_heads, kv_heads)
     how = _check_qk(x, qkv, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    return _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how)
+    _check_upstream(qkv, x, dq_out, dk_out, dv_out)
+    return _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how, _qk_need(how))
 
 
 class _Heads:
     """Where a call's heads lie: tokens ((batch, tokens) or (tokens,)), heads and their size, and q, k and, packed, v as tdm_heads."""
 
     __slots__ = ("tokens", "q_heads", "kv_heads", "dim", "q", "k", "v")
+
+    def alike(self):
+        """Heads of the same number and size, yet to be placed."""
+        x = _Heads()
+        x.tokens, x.q_heads, x.kv_heads, x.dim = self.tokens, self.q_heads, self.kv_heads, self.dim
+        return x
 
 
 def _tensor(t, what):
@@ -340,48 +355,49 @@ def _qk_forward(like, q_weight, k_weight, x, how):
     return q_out, k_out
 
 
-def _upstream(g, x, heads, like, what):
+def _check_upstream(like, x, dq_out, dk_out, dv_out=None):
+    for g, heads, what in ((dq_out, x.q_heads, "dq_out"), (dk_out, x.kv_heads, "dk_out"), (dv_out, x.kv_heads, "dv_out")):
+        if g is not None and (g.dtype != like.dtype or list(g.shape) != [*x.tokens, heads, x.dim] or g.get_device() != like.get_device()):
+            raise ValueError(f"{what}: a gradient of {list(g.shape)} {g.dtype} on {g.device} for {[*x.tokens, heads, x.dim]} {like.dtype} on {like.device}")
+
+
+def _rows(g):
     """An upstream gradient as the kernel reads it: of any strides, the last dimension contiguous."""
-    if g is None:
-        return None
-    if g.dtype != like.dtype or list(g.shape) != [*x.tokens, heads, x.dim] or g.get_device() != like.get_device():
-        raise ValueError(f"{what}: a gradient of {list(g.shape)} {g.dtype} on {g.device} for {[*x.tokens, heads, x.dim]} {like.dtype} on {like.device}")
-    return g if g.stride(-1) == 1 else g.contiguous()
+    return g if g is None or g.stride(-1) == 1 else g.contiguous()
 
 
-def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx):
-    dq_out, dk_out = _upstream(dq_out, x, x.q_heads, like, "dq_out"), _upstream(dk_out, x, x.kv_heads, like, "dk_out")
-    if dx.v is not None:
-        dv_out = _upstream(dv_out, x, x.kv_heads, like, "dv_out")
-    L = lib()
-    need = L.tdm_k6_qk_norm_rope_grad_workspace(how.shape)
+def _qk_need(how):
+    return lib().tdm_k6_qk_norm_rope_grad_workspace(how.shape)
+
+
+def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx, need):
+    dq_out, dk_out, dv_out = _rows(dq_out), _rows(dk_out), _rows(dv_out)
     work = _workspace(need, like)
     dqw, dkw = None if q_weight is None else torch.empty_like(q_weight), None if k_weight is None else torch.empty_like(k_weight)
-    _call(like, L.tdm_k6_qk_norm_rope_grad, how.shape, _view(dq_out), _view(dk_out), _view(dv_out), x.q, x.k, _ptr(q_weight), _ptr(k_weight), how.at(),
-          how.inv_freq.data_ptr(), dx.q, dx.k, dx.v, _ptr(dqw), _ptr(dkw), work.data_ptr(), need)
+    _call(like, lib().tdm_k6_qk_norm_rope_grad, how.shape, _view(dq_out), _view(dk_out), _view(dv_out), x.q, x.k, _ptr(q_weight), _ptr(k_weight),
+          how.at(), how.inv_freq.data_ptr(), dx.q, dx.k, dx.v, _ptr(dqw), _ptr(dkw), work.data_ptr(), need)
     return dqw, dkw
 
 
-def _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how):
+def _separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, how, need):
     dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     dx = _Heads()
     dx.q, dx.k, dx.v = _view(dq), _view(dk), None
-    return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, q_weight, k_weight, x, how, dx))
+    return (dq, dk, *_qk_backward(dq_out, dk_out, None, q, q_weight, k_weight, x, how, dx, need))
 
 
-def _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how):
+def _packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how, need):
     dqkv = qkv.new_empty(qkv.shape)
-    dx = _Heads()
-    dx.q_heads, dx.kv_heads, dx.dim = x.q_heads, x.kv_heads, x.dim
+    dx = x.alike()
     _place_packed(dx, dqkv)
-    return (dqkv, *_qk_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how, dx))
+    return (dqkv, *_qk_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, how, dx, need))
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, x, how):
         ctx.save_for_backward(q, k, q_weight, k_weight, how.positions, how.inv_freq)
-        ctx.how = how.of(None, None)
+        ctx.how, ctx.need = how.of(None, None), _qk_need(how)
         ctx.set_materialize_grads(False)
         return _qk_forward(q, q_weight, k_weight, x, how)
 
@@ -389,14 +405,16 @@ class _QkNormRope(torch.autograd.Function):
     @_once
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
-        return (*_separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, _separate(q, k), ctx.how.of(positions, inv_freq)), None, None)
+        x = _Heads()  # placed anew: hooks on saved tensors may have moved them
+        x.q, x.k = _view(q), _view(k)
+        return (*_separate_backward(dq_out, dk_out, q, k, q_weight, k_weight, x, ctx.how.of(positions, inv_freq), ctx.need), None, None)
 
 
 class _QkvNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, x, how):
         ctx.save_for_backward(qkv, q_weight, k_weight, how.positions, how.inv_freq)
-        ctx.heads, ctx.how = (x.q_heads, x.kv_heads), how.of(None, None)
+        ctx.heads, ctx.how, ctx.need = x.alike(), how.of(None, None), _qk_need(how)
         ctx.set_materialize_grads(False)
         return (*_qk_forward(qkv, q_weight, k_weight, x, how), _values(qkv, x))
 
@@ -404,7 +422,9 @@ class _QkvNormRope(torch.autograd.Function):
     @_once
     def backward(ctx, dq_out, dk_out, dv_out):
         qkv, q_weight, k_weight, positions, inv_freq = ctx.saved_tensors
-        return (*_packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, _packed(qkv, *ctx.heads), ctx.how.of(positions, inv_freq)), None, None)
+        x = ctx.heads.alike()
+        _place_packed(x, qkv)
+        return (*_packed_backward(dq_out, dk_out, dv_out, qkv, q_weight, k_weight, x, ctx.how.of(positions, inv_freq), ctx.need), None, None)
 
 
 # ---- distillation from a teacher's top logits
@@ -481,9 +501,10 @@ def _check_distill(logits, index, teacher, targets, temperature, weight, ignore_
     return how, (index, teacher, targets)
 
 
-def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, upstream, keep_ones):
+def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, upstream, keep_ones, need=None):
     L = lib()
-    need = L.tdm_k7_distill_workspace(how)
+    if need is None:
+        need = L.tdm_k7_distill_workspace(how)
     work = _workspace(need, logits)
     loss = logits.new_empty(logits.shape[:-1] if each_row else (), dtype=torch.float32) if want_loss else None
     _call(logits, L.tdm_k7_distill, how, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), _ptr(targets), _ptr(loss), _ptr(grad),
@@ -495,10 +516,10 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, targets, how, each_row):
         ctx.save_for_backward(logits, index, teacher, targets)
-        ctx.how, ctx.each_row = how, each_row
+        ctx.how, ctx.each_row, ctx.need = how, each_row, lib().tdm_k7_distill_workspace(how)
         # float16 is trained with a scaled loss: a gradient computed here would be for nothing
         ctx.grad = None if logits.dtype == torch.float16 else _empty_at_phase_of(logits)
-        return _distill(logits, index, teacher, targets, how, each_row, True, ctx.grad, None, False)
+        return _distill(logits, index, teacher, targets, how, each_row, True, ctx.grad, None, False, ctx.need)
 
     @staticmethod
     @_once
@@ -509,5 +530,5 @@ class _Distill(torch.autograd.Function):
         first = grad is not None
         if not first:
             grad = _empty_at_phase_of(ctx.saved_tensors[0])
-        _distill(*ctx.saved_tensors, ctx.how, ctx.each_row, False, grad, upstream.contiguous(), first)
+        _distill(*ctx.saved_tensors, ctx.how, ctx.each_row, False, grad, upstream if upstream.is_contiguous() else upstream.contiguous(), first, ctx.need)
         return grad, None, None, None, None, None
