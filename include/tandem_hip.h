@@ -373,7 +373,7 @@ int tdm_k4_unit_gather_all(void* const* fulls, const void* const* shards, const 
  * workspace of the caller's, which it may fill with anything, and which two launches that can run at the same time must not share.
  *
  * out[i, :] = scale * weight[tokens[i], :] for i < n; weight [vocab, dim], out [n, dim], both contiguous; at most 2^28 tokens and 2^24 rows. Tokens are
- * TDM_I64 or TDM_I32 (index_dtype). A token outside [0, vocab) reads nothing; its row of out is NaN. */
+ * TDM_I64 or TDM_I32 (index_dtype). A token outside [0, vocab) reads nothing outside the table; its row of out is NaN. */
 int tdm_k5_embedding(const void* weight, const void* tokens, int index_dtype, void* out, int64_t n, int64_t vocab, int64_t dim, int dtype,
                      float scale, tdm_stream stream);
 
@@ -413,7 +413,7 @@ typedef struct tdm_qk_shape {
 /* Every query and key head x becomes y = x / sqrt(mean(x^2) + eps) * weight (weight [head_dim]; NULL: ones), then every pair
  * (a, b) of its rotated elements (a cos - b sin, b cos + a sin) of the angle position * inv_freq[i], i the pair's number (inv_freq:
  * rotary_dim / 2 doubles in GPU memory; the angle is computed in doubles). One pass: x read once, y written once. q_out may be q
- * and k_out may be k. */
+ * and k_out may be k. A call that would take 2^24 workgroups (a workgroup takes up to 32 tokens) is refused. */
 int tdm_k6_qk_norm_rope(const tdm_qk_shape* shape, const tdm_heads* q, const tdm_heads* k, const void* q_weight, const void* k_weight,
                         const tdm_positions* positions, const double* inv_freq, const tdm_heads* q_out, const tdm_heads* k_out,
                         tdm_stream stream);
@@ -456,7 +456,7 @@ typedef struct tdm_distill_how {
  * of scale * upstream * loss with respect to the logits, rounded once. upstream (fp32 in GPU memory: one value, or [rows]
  * with TDM_DISTILL_NONE) may be NULL: ones. With keep_ones the gradient of the rows whose upstream is 1 is left as it is: a caller that
  * has it from an earlier call computes only what an upstream value changes. A teacher's entry with a negative column or a logit of
- * -inf says nothing; a row without another has no first term; entries of the same column add up. A column, or a target that
+ * -inf says nothing (the teacher's logits take no gradient); a row without another has no first term; entries of the same column add up. A column, or a target that
  * is used, outside the vocabulary and a NaN among the teacher's logits make the row's loss and gradient NaN; nothing is read there.
  * logits is contiguous; grad starts at the same distance from a 16-byte boundary as logits. The workspace starts
  * on 16 bytes and holds tdm_k7_distill_workspace(how) bytes (-1: arguments out of range). Sums have a fixed order. */

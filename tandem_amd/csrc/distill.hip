@@ -173,7 +173,8 @@ constexpr uint32_t kNoColumn = 0xffffffffu;
 // exponentials are taken as the vectors arrive, and one barrier joins the waves. While the gradient of a row is computed, each of
 // its vectors makes room for the next row's: loads, exponentials and stores are under way at the same time with one workgroup per
 // compute unit. The teacher's entries are one lane's each (k <= kG): their elements and the target's are written again after the row, behind
-// a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries.
+// a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries. 8192 rows of 131072 bf16
+// logits and their gradient take 806 us, 5.3 TB/s: bound by memory, reads and writes mixed (797 us with the exponentials taken out).
 template <typename T, int kG, int kHeld, Mix kMix>
 __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_table) {
   constexpr int kN = per_vec<T>(), kWaves = kG / kWave;
@@ -472,7 +473,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
 }
 
 // Short rows: 16 lanes a row, so that what a row needs once is done for four rows by every instruction of a wave (8192 rows of 256
-// floats, 16 entries, two temperatures: 14.1 us with a wave a row). kHeld vectors of the row and kEntries of the teacher's entries per lane.
+// floats, 16 entries, two temperatures: 11.2 us; 14.1 with a wave a row). kHeld vectors of the row and kEntries of the teacher's entries per lane.
 constexpr int kShortLanes = 16, kShortThreads = 256, kShortRows = kShortThreads / kShortLanes;
 
 template <typename T, int kHeld, int kEntries, Mix kMix>
@@ -649,7 +650,7 @@ __global__ __launch_bounds__(kFoldThreads) void distill_sum_kernel(DistillArgs a
 }
 
 // The loss alone of a few long rows: with a workgroup per row most compute units are idle (4 rows of 131072 bf16 logits: 14.2 us and the
-// sum's launch). Every row is split over `slices` workgroups, which leave their maximum and sums; one more workgroup joins them, a wave
+// sum's launch; split, 3.6 and 3.6). Every row is split over `slices` workgroups, which leave their maximum and sums; one more workgroup joins them, a wave
 // per row, with the teacher's share.
 constexpr int kSliceThreads = 256, kMostSlices = kWave;
 

@@ -43,6 +43,9 @@ struct LookupArgs {
   float scale;
 };
 
+// A copy with a product, bound by memory: 32768 rows of 2048 bf16 take 39 us, 6.9 TB/s of rows read and written. As many lanes as a row has
+// accesses, up to a workgroup; four rows of each are under way at once, since a row's address waits for its token. One row:
+// 3.3 us, the launch.
 template <typename T, typename I, int kBytes>
 __global__ __launch_bounds__(kLookupThreads) void embedding_lookup_kernel(LookupArgs a) {
   constexpr int kN = kBytes / static_cast<int>(sizeof(T));
@@ -130,8 +133,8 @@ __device__ __forceinline__ void write_zeros(void* base, int64_t bytes, int64_t b
 // of each token go, and places them in the order in which they come: a wave walks its stretch of tokens 64 at a
 // time, and for every distinct token of its share among the 64 moves that token's counter on once. Any skew is right, and the
 // result is the same every time. A lane reads kHeld tokens at once; where they are all its tokens, they stay in registers for
-// the second walk. (A radix sort of 8192 tokens in one workgroup's LDS took 12.6 us for 8192 byte tokens, its
-// merge of four such tiles another 12: one compute unit's instruction rate bound it.)
+// the second walk. 8192 byte tokens: 10.5 us, bound by the chain of walks, counters and barriers, not by memory. (A radix sort of
+// them in one workgroup's LDS took 12.6 us, its merge of four such tiles another 12: one compute unit's instruction rate bound it.)
 template <typename I, int kHeld>
 __global__ __launch_bounds__(kSortThreads, 8) void embedding_sort_kernel(SortArgs a) {
   if (blockIdx.x >> a.log_shares != 0) {
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(kSortThreads, 8) void embedding_sort_kernel(SortArg
 }
 
 // The same result for many tokens, each read by one workgroup instead of by all (32768 int64 tokens of a vocabulary of 131072: 25 us by 256
-// workgroups that all read them, most of it waiting for the same lines). A tile of tokens is brought in order of their shares, `from`
+// workgroups that all read them, most of it waiting for the same lines; a training step of 2048 columns took 194 us with that, 181 with the split). A tile of tokens is brought in order of their shares, `from`
 // where they came from; offsets[tile][share]: where the share's begin in the tile.
 constexpr int kSplitThreads = 512, kSplitWaves = kSplitThreads / kWave, kSplitItems = 2, kTile = kSplitThreads * kSplitItems;
 constexpr int kPlaceItems = 4;
@@ -506,6 +509,9 @@ __device__ void zero_rows(const SumArgs& a) {
   }
 }
 
+// Bound by memory where the table is large: 32768 rows of 2048 bf16 into 131072, 134 MB read and 439 MB written here, take 103 us, 5.6 TB/s.
+// Eight rows of g are under way per wave. Chunks of equal length, not one token's rows each: byte tokens, some of which come
+// hundreds of times, keep every wave busy (8192 x 512 fp32 for 256 tokens: 6.8 us for 17 MB, and 4.7 for the join).
 template <typename T, int kBytes>
 __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(SumArgs a) {
   constexpr int kN = kBytes / static_cast<int>(sizeof(T));

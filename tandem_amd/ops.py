@@ -90,7 +90,7 @@ def _padding(padding_idx, vocab):
 def embedding(tokens, weight, scale=1.0, padding_idx=None):
     """scale * weight[tokens]: tokens of any shape (int64 or int32), weight [vocab, dim] contiguous; the result has the tokens'
     shape and dim behind it, in weight's dtype. `padding_idx`: a token whose row takes no gradient. A token outside
-    [0, vocab) reads nothing: its row comes out as NaN, and takes no gradient.
+    [0, vocab) comes out as a row of NaN, and takes no gradient.
 
     The gradient of weight is dense and written in one pass over the upstream gradient, its rows added in the order of
     the tokens (see embedding_grad)."""
