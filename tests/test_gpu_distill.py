@@ -324,6 +324,21 @@ def test_an_upstream_gradient_other_than_one():
     assert torch.equal(got[0::4], ones[0::4]) and (got[2::4] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_scaled_loss_s_gradient_is_that_of_the_scale(dtype, reduction):
+    """Loss scaling through autograd, for every type the bits of a call that is given the scale (a power of two); and again, retained."""
+    from tandem_amd import ops
+
+    for rows, vocab in ((40, 300), (70, 9001)):
+        x, idx, t, y = make(rows, vocab, 7, dtype, 23, ignored=0.2)
+        leaf = x.clone().requires_grad_()
+        loss = ops.distill_loss(leaf, idx, t, y, temperature=2.0, weight=0.5, reduction=reduction)
+        for scale in (4096.0, 1.0, -2.0):
+            (got,) = torch.autograd.grad(loss.sum() * scale, leaf, retain_graph=True)
+            assert torch.equal(got, ops.distill_loss_and_grad(x, idx, t, y, temperature=2.0, weight=0.5, reduction=reduction, scale=scale)[1]), (rows, scale)
+
+
 def test_gradient_against_differences():
     """Central differences of the loss in fp32, step 2^-5 on logits of order 3: the third-order term is below h^2 / 6 times the third
     derivative, under 2 per row: 2^-11; the rounding of a loss below 16 (2^-20) over the step's 2^-4: 2^-16 each."""
