@@ -380,7 +380,7 @@ int tdm_k5_embedding(const void* weight, const void* tokens, int index_dtype, vo
 /* dweight[v, :] = scale * the sum of grad[i, :] over the i with tokens[i] = v, in the order of i, summed in fp32 and rounded
  * once: the same bits every time. All of dweight [vocab, dim] is written; a row without a token is zero. The token
  * `padding` (-1: none) and tokens outside [0, vocab) take no gradient. The workspace starts on 16 bytes and holds
- * tdm_k5_embedding_grad_workspace(n, vocab, dim) bytes (-1: arguments out of range). */
+ * tdm_k5_embedding_grad_workspace(n, vocab, dim) bytes (-1: arguments out of range; 0: none, it may be NULL). */
 int64_t tdm_k5_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t dim);
 int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype, void* dweight, void* workspace, int64_t workspace_bytes,
                           int64_t n, int64_t vocab, int64_t dim, int dtype, float scale, int64_t padding, tdm_stream stream);

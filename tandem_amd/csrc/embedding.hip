@@ -13,6 +13,7 @@
 //      the chunk is finished there; one that crosses the chunk's ends leaves fp32 partial sums. The launch's other workgroups
 //      write the zeros of the rows that have no token (most rows of a large vocabulary).
 //   3. embedding_join_kernel: adds the partial sums of the tokens that cross chunks, in order.
+// Small tables and few tokens: embedding_row_kernel alone.
 
 #include <hip/hip_runtime.h>
 
@@ -637,9 +638,114 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void embedding_join_kernel(SumAr
   static_cast<T*>(a.dweight)[static_cast<int64_t>(key) * a.dim + c] = narrow<T>(sum * a.scale);
 }
 
+// ---------------------------------------------------------------- small tables
+
+// The whole gradient in one launch, for few rows and tokens: a workgroup per row of dW and slice of its columns reads all tokens, lists the places of
+// its own in order, and adds those rows of g, a group of lanes per stretch of the list and the groups' sums in order. A row without a token
+// comes out as zeros. Latency bounds it, and with it how often the commonest token comes, since one workgroup's loads add it up: 256 rows
+// of 512 floats take 5.3 us for 256 tokens, 7.9 for 4096 and 8.8 with a quarter of them the same (sort, sums and join: 10.8, 12.2 and 12.6).
+// 8192 tokens, with twice the steps: 11.5 and 15.0 (16.5 and 17.9), but rows that allow no wide loads 26 (21). With 2048 workgroups
+// instead of at most 1024 what every one of them costs shows: 512 rows of 512 floats, 4096 tokens, 14.0 us (12.6).
+constexpr int kRowThreads = 512, kRowWaves = kRowThreads / kWave, kRowSteps = 8;
+constexpr int kRowTokens = kRowThreads * kRowSteps;
+
+struct RowArgs {
+  const void *grad, *tokens;
+  void* dweight;
+  int64_t dim;
+  uint32_t n, per_wave, padding;
+  int slices, vecs, log_lanes;
+  float scale;
+};
+
+template <typename T, typename I, int kBytes>
+__global__ __launch_bounds__(kRowThreads) void embedding_row_kernel(RowArgs a) {
+  constexpr int kN = kBytes / static_cast<int>(sizeof(T)), kAhead = kBytes >= 8 ? 16 : 32;
+  using P = Pack<T, kN>;
+  using Sums = Pack<float, kN < 4 ? kN : 4>;
+  __shared__ uint16_t s_list[kRowTokens];
+  __shared__ uint32_t s_found[kRowWaves];
+  __shared__ __attribute__((aligned(16))) float s_acc[kRowThreads * kN];
+  const uint32_t tid = threadIdx.x, lane = tid % kWave;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const uint32_t v = blockIdx.x / static_cast<uint32_t>(a.slices), slice = blockIdx.x - v * static_cast<uint32_t>(a.slices);
+  const uint32_t first = wave * a.per_wave;
+  uint32_t mine = 0, found = 0;  // bit j: this lane's token of step j is the row's
+#pragma unroll
+  for (uint32_t j = 0; j < kRowSteps; ++j) {
+    const uint32_t n = first + j * kWave + lane;
+    if (j * kWave < a.per_wave && n < a.n && static_cast<const I*>(a.tokens)[n] == static_cast<I>(v)) mine |= 1u << j;
+  }
+  if (v == a.padding) mine = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < kRowSteps; ++j) found += static_cast<uint32_t>(__popcll(__ballot((mine >> j) & 1)));
+  if (lane == 0) s_found[wave] = found;
+  __syncthreads();
+  uint32_t at = 0, all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kRowWaves; ++w) {
+    if (w < wave) at += s_found[w];
+    all += s_found[w];
+  }
+  if (found != 0) {
+#pragma unroll
+    for (uint32_t j = 0; j < kRowSteps; ++j) {
+      const uint64_t votes = __ballot((mine >> j) & 1);
+      if ((mine >> j) & 1) s_list[at + static_cast<uint32_t>(__popcll(votes & ((1ull << lane) - 1)))] = static_cast<uint16_t>(first + j * kWave + lane);
+      at += static_cast<uint32_t>(__popcll(votes));
+    }
+  }
+  __syncthreads();
+
+  const uint32_t lanes = 1u << a.log_lanes, group = tid >> a.log_lanes, groups = kRowThreads >> a.log_lanes;
+  const uint32_t vec = slice * lanes + (tid & (lanes - 1));
+  const uint32_t per = std::max(1u, (all + groups - 1) / groups), used = (all + per - 1) / per;  // groups that have entries
+  const uint32_t end = std::min((group + 1) * per, all);
+  float acc[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) acc[i] = 0.0f;
+  if (vec < static_cast<uint32_t>(a.vecs)) {
+    const T* const grad = static_cast<const T*>(a.grad) + static_cast<int64_t>(vec) * kN;
+    uint32_t e = group * per;
+    auto add = [&](auto ahead, uint32_t count) {  // the next `count` entries, all under way at once
+      P row[ahead.value];
+#pragma unroll
+      for (uint32_t u = 0; u < ahead.value; ++u) row[u] = P::load(grad + static_cast<int64_t>(s_list[e + std::min(u, count - 1)]) * a.dim);
+#pragma unroll
+      for (uint32_t u = 0; u < ahead.value; ++u)
+        if (u < count) {
+          float f[kN];
+          row[u].get(f);
+#pragma unroll
+          for (int i = 0; i < kN; ++i) acc[i] += f[i];
+        }
+      e += count;
+    };
+    while (e + kAhead <= end) add(std::integral_constant<int, kAhead>{}, kAhead);
+    while (e < end) add(std::integral_constant<int, 4>{}, std::min(4u, end - e));
+  }
+#pragma unroll
+  for (int i = 0; i < kN; i += 4) {
+    Sums p;
+    p.set(acc + i);
+    p.store(s_acc + tid * kN + i);
+  }
+  __syncthreads();
+  const uint32_t cols = lanes * kN;
+  const int64_t col = static_cast<int64_t>(slice) * cols + tid;
+  if (tid >= cols || col >= a.dim) return;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (uint32_t g = 0; g < used; ++g) sum += s_acc[g * cols + tid];
+  static_cast<T*>(a.dweight)[static_cast<int64_t>(v) * a.dim + col] = narrow<T>(sum * a.scale);
+}
+
 // ---------------------------------------------------------------- host
 
 constexpr int64_t kMostTokens = int64_t(1) << 28;  // the sums' launch stays below 2^32 lanes
+
+// Whether a gradient is the one launch's: at most 1024 workgroups, a row's 512 bytes each.
+bool one_launch(int64_t n, int64_t vocab, int64_t dim, int es) { return n <= kRowTokens && vocab * ((dim * es + 511) / 512) <= 1024; }
 
 constexpr int64_t kMostVocab = int64_t(1) << 24;  // 2^14 workgroups place the tokens
 
@@ -692,6 +798,7 @@ Workspace workspace_of(int64_t n, int64_t vocab, int64_t dim) {
     w.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
+  if (one_launch(n, vocab, dim, 4)) return w;  // and of any type's
   w.log_shares = log_shares_of(vocab);
   w.share = ((vocab - 1) >> w.log_shares) + 1;
   w.pitch = (dim + 3) / 4 * 4;
@@ -767,11 +874,32 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     check_index(index_dtype);
     require(dweight != nullptr && (n == 0 || (grad != nullptr && tokens != nullptr)), "embedding_grad: null pointer");
     const Workspace ws = workspace_of(n, vocab, dim);
-    require(workspace != nullptr && workspace_bytes >= ws.bytes, "embedding_grad: the workspace is smaller than tdm_k5_embedding_grad_workspace says");
+    require(ws.bytes == 0 || (workspace != nullptr && workspace_bytes >= ws.bytes), "embedding_grad: the workspace is smaller than tdm_k5_embedding_grad_workspace says");
     require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "embedding_grad: the workspace must start on 16 bytes");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* const base = static_cast<char*>(workspace);
     const int es = dtype == TDM_F32 ? 4 : 2;
+    const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
+    const int vecs = static_cast<int>(dim * es / width);
+    const uint32_t padding_row = padding >= 0 && padding < vocab ? static_cast<uint32_t>(padding) : kNoToken;
+    if (one_launch(n, vocab, dim, es)) {
+      RowArgs a{grad, tokens, dweight, dim, static_cast<uint32_t>(n), static_cast<uint32_t>((n + kRowThreads - 1) / kRowThreads * kWave), padding_row, 0, vecs, 3, scale};
+      // 8 lanes or more side by side, up to 32, and as many more as 128 columns take
+      while ((1 << a.log_lanes) < vecs && (a.log_lanes < 5 || (width / es << a.log_lanes) < 128)) ++a.log_lanes;
+      a.slices = (vecs + (1 << a.log_lanes) - 1) >> a.log_lanes;
+      const dim3 grid(static_cast<unsigned>(vocab * a.slices));
+      with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        with_width(width, [&](auto w) {
+          if constexpr (w.value >= static_cast<int>(sizeof(T))) {
+            if (index_dtype == TDM_I64) hipLaunchKernelGGL((embedding_row_kernel<T, int64_t, w.value>), grid, dim3(kRowThreads), 0, st, a);
+            else hipLaunchKernelGGL((embedding_row_kernel<T, int32_t, w.value>), grid, dim3(kRowThreads), 0, st, a);
+          }
+        });
+      });
+      check_launch("embedding_row launch");
+      return;
+    }
 
     SortArgs s{};
     s.tokens = tokens;
@@ -779,7 +907,7 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     s.order = reinterpret_cast<uint32_t*>(base + ws.order);
     s.starts = reinterpret_cast<uint32_t*>(base + ws.starts);
     s.vocab = static_cast<uint32_t>(vocab);
-    s.padding = padding >= 0 && padding < vocab ? static_cast<uint32_t>(padding) : kNoToken;
+    s.padding = padding_row;
     s.n = static_cast<uint32_t>(n);
     s.per_wave = static_cast<uint32_t>((n + kSortThreads - 1) / kSortThreads * kWave);
     s.share = static_cast<uint32_t>(ws.share);
@@ -792,7 +920,6 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     while (hidden * row_bytes % 16 != 0) --hidden;
     s.zero = dweight;
     s.zero_bytes = hidden * row_bytes;
-    const int width = access_width(reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(dweight) | static_cast<uintptr_t>(dim * es), es);
     SumArgs a{};
     a.grad = grad;
     a.keys = s.keys;
@@ -807,7 +934,7 @@ int tdm_k5_embedding_grad(const void* grad, const void* tokens, int index_dtype,
     a.log_shares = s.log_shares;
     a.all = s.share << s.log_shares;
     a.chunk = chunk_of(n, dim);
-    a.vecs = static_cast<int>(dim * es / width);
+    a.vecs = vecs;
     a.slices = (a.vecs + kWave - 1) / kWave;
     a.zero_from = hidden;
     a.zero_rows = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kZeroRows, kZeroBytes / row_bytes)));

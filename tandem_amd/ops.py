@@ -62,7 +62,7 @@ def _call(t, entry, *args):
 def _workspace(bytes_needed, like):
     if bytes_needed < 0:
         raise ValueError(lib().tdm_last_error().decode(errors="replace"))
-    return like.new_empty(bytes_needed, dtype=torch.uint8)
+    return like.new_empty(bytes_needed, dtype=torch.uint8) if bytes_needed else None
 
 
 def _once(backward):
@@ -140,7 +140,7 @@ def _embedding_grad(grad, tokens, vocab, scale, padding):
 def _embedding_backward(grad, tokens, vocab, dim, scale, padding, need):
     out = grad.new_empty((vocab, dim))
     work = _workspace(need, grad)
-    _call(grad, lib().tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), work.data_ptr(), need,
+    _call(grad, lib().tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), _ptr(work), need,
           tokens.numel(), vocab, dim, CODES[grad.dtype], scale, padding)
     return out
 
@@ -375,7 +375,7 @@ def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx, n
     work = _workspace(need, like)
     dqw, dkw = None if q_weight is None else torch.empty_like(q_weight), None if k_weight is None else torch.empty_like(k_weight)
     _call(like, lib().tdm_k6_qk_norm_rope_grad, how.shape, _view(dq_out), _view(dk_out), _view(dv_out), x.q, x.k, _ptr(q_weight), _ptr(k_weight),
-          how.at(), how.inv_freq.data_ptr(), dx.q, dx.k, dx.v, _ptr(dqw), _ptr(dkw), work.data_ptr(), need)
+          how.at(), how.inv_freq.data_ptr(), dx.q, dx.k, dx.v, _ptr(dqw), _ptr(dkw), _ptr(work), need)
     return dqw, dkw
 
 
@@ -508,7 +508,7 @@ def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, up
     work = _workspace(need, logits)
     loss = logits.new_empty(logits.shape[:-1] if each_row else (), dtype=torch.float32) if want_loss else None
     _call(logits, L.tdm_k7_distill, how, logits.data_ptr(), index.data_ptr(), teacher.data_ptr(), _ptr(targets), _ptr(loss), _ptr(grad),
-          _ptr(upstream), int(keep_ones), work.data_ptr(), need)
+          _ptr(upstream), int(keep_ones), _ptr(work), need)
     return loss
 
 

@@ -174,6 +174,22 @@ def test_every_way_of_sorting(vocab, n, kind):
     assert torch.equal(got, ops.embedding_grad(grad.to(DEV), tokens.to(DEV), vocab))
 
 
+@pytest.mark.parametrize("vocab,dim,dtype", [(1024, 128, torch.float32), (1025, 128, torch.float32), (256, 512, torch.float32), (341, 384, torch.float16),
+                                             (512, 512, torch.bfloat16), (513, 512, torch.bfloat16), (97, 511, torch.bfloat16), (300, 33, torch.float32),
+                                             (5, 6, torch.float16), (1, 1, torch.float32)])
+@pytest.mark.parametrize("n,kind", [(1, "text"), (63, "same"), (64, "distinct"), (513, "outside"), (4095, "same"), (4096, "text"), (4097, "text")])
+def test_small_tables(vocab, dim, dtype, n, kind):
+    """Both sides of the sizes where one launch does it all: 4096 tokens, 1024 rows of 512 bytes; narrow and wide accesses, a padding row."""
+    from tandem_amd import ops
+
+    tokens = make_tokens(kind, n, vocab, 14)
+    grad = torch.randn(n, dim, generator=torch.Generator().manual_seed(15)).to(dtype)
+    for padding, index in ((None, torch.int64), (int(tokens[0]) if 0 <= int(tokens[0]) < vocab else 0, torch.int32)):
+        got = ops.embedding_grad(grad.to(DEV), tokens.to(index).to(DEV), vocab, scale=0.5, padding_idx=padding)
+        check_grad(got, grad, tokens, vocab, 0.5, padding)
+        assert torch.equal(got, ops.embedding_grad(grad.to(DEV), tokens.to(index).to(DEV), vocab, scale=0.5, padding_idx=padding))
+
+
 def test_more_tokens_than_the_tiles_of_a_split():
     from tandem_amd import ops
 
