@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
   constexpr int kAhead = 4;          // vectors in flight of a row that is read twice, or for its loss alone
   constexpr int kEarly = kHeld / 2;  // vectors of the next row that are read while this row's gradient is written
   Vec16 held[kHeld > 0 ? kHeld : 1];
-  __amdgpu_buffer_rsrc_t from = stretch(nullptr, 0);
+  Stretch from = stretch(nullptr, 0);
   T edge_held = narrow<T>(0.0f);
   uint32_t col = kNoColumn;  // of the teacher's entry of this lane
   float t = -__builtin_inff();
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     const bool held_fits = sizeof(T) == 4 || (fabsf(base * c) < 1024.0f && (kMix != kTwo || fabsf(base * kLog2e) < 1024.0f));
     if constexpr (kHeld > 0) {
       from = stretch(nx + next_body.head, next < a.rows ? next_body.vecs * 16 : 0);
-      const __amdgpu_buffer_rsrc_t to = stretch(g + body.head, g != nullptr && !idle && held_fits ? body.vecs * 16 : 0);
+      const Stretch to = stretch(g + body.head, g != nullptr && !idle && held_fits ? body.vecs * 16 : 0);
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         if (g != nullptr) {

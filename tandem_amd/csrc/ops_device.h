@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <limits>
 #include <string>
@@ -95,18 +96,24 @@ __device__ __forceinline__ Vec16 pack16(const float (&f)[per_vec<T>()]) {
 }
 
 // A stretch of memory for buffer accesses: one register of offsets for many accesses (the rest of an address is scalar), loads
-// behind its end give zeros and stores there do nothing.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t stretch(const void* base, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);  // raw, 32-bit elements
+// behind its end give zeros and stores there do nothing. Only the vector operand is promised to be compared with the end, so the
+// scalar part of an offset moves the stretch's beginning and shortens it; the instruction's own scalar operand stays zero.
+struct Stretch {
+  char* base;
+  int bytes;
+};
+__device__ __forceinline__ Stretch stretch(const void* base, int bytes) { return Stretch{static_cast<char*>(const_cast<void*>(base)), bytes}; }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t behind(const Stretch& s, int offset) {
+  return __builtin_amdgcn_make_buffer_rsrc(s.base + offset, 0, std::max(s.bytes - offset, 0), 0x00027000);  // raw, 32-bit elements
 }
 constexpr int kPlain = 0, kStream = 2;  // cache policies: cached; non-temporal
 template <int kPolicy>
-__device__ __forceinline__ Vec16 load16(__amdgpu_buffer_rsrc_t from, int lane_offset, int offset) {
-  return __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, kPolicy);
+__device__ __forceinline__ Vec16 load16(const Stretch& from, int lane_offset, int offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(behind(from, offset), lane_offset, 0, kPolicy);
 }
 template <int kPolicy>
-__device__ __forceinline__ void store16(const Vec16& v, __amdgpu_buffer_rsrc_t to, int lane_offset, int offset) {
-  __builtin_amdgcn_raw_buffer_store_b128(v, to, lane_offset, offset, kPolicy);
+__device__ __forceinline__ void store16(const Vec16& v, const Stretch& to, int lane_offset, int offset) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, behind(to, offset), lane_offset, 0, kPolicy);
 }
 
 // Reductions over the 64 lanes of a wave by DPP: sums along the rows of 16 lanes, then rows 0 and 2 into 1 and 3, then the lower
