@@ -2,7 +2,7 @@
 gradient by sorted tokens; the norms of queries and keys per head with the position rotation in the same pass;
 the distillation loss from a teacher's top logits with its gradient.
 
-Functions on tensors in GPU memory, differentiable, launched on the current stream of the tensors' device; float32,
+Functions on tensors in GPU memory, differentiable (in reverse mode, once), launched on the current stream of the tensors' device; float32,
 float16 and bfloat16, sums in fp32, one rounding at the end. Each has its gradient beside it (`*_grad`) for programs that
 run their backward pass by hand. Nothing here waits for the GPU, every result is the same bits every time, and all of it can be
 captured into a graph. The reference has no counterpart: its model (tandem/model.py:14-120 there) is made of torch's own
@@ -12,6 +12,7 @@ operators.
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import DISTILL_HOW, DTYPES as CODES, HEADS, POSITIONS, QK_SHAPE, check, lib, require_device_tensor
 
@@ -24,10 +25,24 @@ def _on_gpu(t, what):
         raise ValueError(f"{what}: needs a tensor in GPU memory (got {getattr(t, 'device', type(t))}); tandem_amd has no CPU path")
 
 
-def _floating(t, what):
+def _no_tangent(*tensors):
+    """Refuses operands that carry a tangent of forward-mode differentiation: the kernels would drop it, and the result's derivative be zero."""
+    if forward_ad._current_level < 0:  # no level is open: no tensor has one
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("tandem_amd.ops has no derivatives in forward mode")
+
+
+def _tensor(t, what):
     _on_gpu(t, what)
     if t.dtype not in DTYPES:
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
+    _no_tangent(t)
+
+
+def _floating(t, what):
+    _tensor(t, what)
     if not t.is_contiguous():
         raise ValueError(f"{what}: needs a contiguous tensor")
 
@@ -138,6 +153,7 @@ def _embedding_grad(grad, tokens, vocab, scale, padding):
 
 
 def _embedding_backward(grad, tokens, vocab, dim, scale, padding, need):
+    _no_tangent(grad)
     out = grad.new_empty((vocab, dim))
     work = _workspace(need, grad)
     _call(grad, lib().tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), _ptr(work), need,
@@ -233,12 +249,6 @@ class _Heads:
         return x
 
 
-def _tensor(t, what):
-    _on_gpu(t, what)
-    if t.dtype not in DTYPES:
-        raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
-
-
 def _packed(qkv, q_heads, kv_heads):
     _tensor(qkv, "qkv")
     *tokens, width = qkv.shape
@@ -325,6 +335,7 @@ def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved
     if not isinstance(positions, torch.Tensor) or positions.dtype not in INDEX_DTYPES:
         raise ValueError("positions: an int64 or int32 tensor")
     require_device_tensor(inv_freq, "qk_norm_rope(inv_freq)")
+    _no_tangent(inv_freq)
     rotary = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or rotary > x.dim:
         raise ValueError(f"inv_freq: at most {x.dim // 2} float64 values")
@@ -371,6 +382,7 @@ def _qk_need(how):
 
 
 def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx, need):
+    _no_tangent(dq_out, dk_out, dv_out)
     dq_out, dk_out, dv_out = _rows(dq_out), _rows(dk_out), _rows(dv_out)
     work = _workspace(need, like)
     dqw, dkw = None if q_weight is None else torch.empty_like(q_weight), None if k_weight is None else torch.empty_like(k_weight)
@@ -524,6 +536,7 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, upstream):
+        _no_tangent(upstream)
         # the gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out
         # once; a second backward pass through the same graph computes its own.
         grad, ctx.grad = ctx.grad, None

@@ -1,0 +1,93 @@
+"""What the model operators do around their launches, on the CPU: the launches are replaced by nothing, the rest is as on the GPU."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+
+class NoLaunches:
+    """The library, its kernels left out: every launch is noted with its arguments."""
+
+    def __init__(self, library):
+        self.library, self.calls = library, []
+
+    def __getattr__(self, name):
+        if not name.startswith("tdm_k") or name.endswith("_workspace"):
+            return getattr(self.library, name)
+
+        def launch(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return launch
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    from tandem_amd import ops
+
+    stand_in = NoLaunches(ops.lib())
+    monkeypatch.setattr(ops, "lib", lambda: stand_in)
+    monkeypatch.setattr(ops, "_on_gpu", lambda t, what: None)
+    monkeypatch.setattr(ops, "require_device_tensor", lambda t, what: None)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)  # a CPU tensor's get_device()
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
+    return stand_in.calls
+
+
+def operands():
+    """The operands of every operator and of its gradient, by name."""
+    from tandem_amd import ops
+
+    tokens, positions = torch.tensor([1, 2, 1]), torch.arange(3)
+    w, g = torch.randn(5, 8), torch.randn(3, 8)
+    q, k, v, qkv = torch.randn(1, 3, 2, 8), torch.randn(1, 3, 1, 8), torch.randn(1, 3, 1, 8), torch.randn(1, 3, 32)
+    qw, kw, freq = torch.randn(8), torch.randn(8), ops.rope_frequencies(8, device="cpu")
+    x, t, columns, y = torch.randn(3, 9), torch.randn(3, 2), torch.zeros(3, 2, dtype=torch.int64), torch.tensor([1, 2, 3])
+    return {
+        "embedding": (lambda w: ops.embedding(tokens, w), dict(w=w)),
+        "embedding_grad": (lambda g: ops.embedding_grad(g, tokens, 5), dict(g=g)),
+        "qk_norm_rope": (lambda q, k, qw, kw, freq: ops.qk_norm_rope(q, k, qw, kw, positions, freq), dict(q=q, k=k, qw=qw, kw=kw, freq=freq)),
+        "qk_norm_rope_grad": (lambda dq, dk, q, k, qw, kw, freq: ops.qk_norm_rope_grad(dq, dk, q, k, qw, kw, positions, freq),
+                              dict(dq=q.clone(), dk=k.clone(), q=q, k=k, qw=qw, kw=kw, freq=freq)),
+        "qkv_norm_rope": (lambda qkv, qw, kw, freq: ops.qkv_norm_rope(qkv, 2, 1, qw, kw, positions, freq), dict(qkv=qkv, qw=qw, kw=kw, freq=freq)),
+        "qkv_norm_rope_grad": (lambda dq, dk, dv, qkv, qw, kw, freq: ops.qkv_norm_rope_grad(dq, dk, dv, qkv, 2, 1, qw, kw, positions, freq),
+                               dict(dq=q.clone(), dk=k.clone(), dv=v, qkv=qkv, qw=qw, kw=kw, freq=freq)),
+        "distill_loss": (lambda x, t: ops.distill_loss(x, columns, t, targets=y, weight=0.5), dict(x=x, t=t)),
+        "distill_loss_and_grad": (lambda x, t: ops.distill_loss_and_grad(x, columns, t, targets=y, weight=0.5), dict(x=x, t=t)),
+    }
+
+
+NAMES = ["embedding", "embedding_grad", "qk_norm_rope", "qk_norm_rope_grad", "qkv_norm_rope", "qkv_norm_rope_grad", "distill_loss", "distill_loss_and_grad"]
+DIFFERENTIABLE = ["embedding", "qk_norm_rope", "qkv_norm_rope", "distill_loss"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_derivatives_are_refused(launches, name):
+    """An operand with a tangent would come out without one: a derivative of zero."""
+    call, given = operands()[name]
+    with forward_ad.dual_level():
+        call(**given)  # no tangents, no refusal
+        for which in given:
+            done = len(launches)
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call(**{**given, which: forward_ad.make_dual(given[which], torch.ones_like(given[which]))})
+            assert len(launches) == done, which
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+                call(**{**given, which: forward_ad.make_dual(given[which], torch.ones_like(given[which]))})
+
+
+@pytest.mark.parametrize("name", DIFFERENTIABLE)
+def test_an_upstream_gradient_with_a_tangent_is_refused(launches, name):
+    call, given = operands()[name]
+    first = next(iter(given))
+    out = call(**{**given, first: given[first].clone().requires_grad_()})
+    out = out if isinstance(out, torch.Tensor) else out[0]
+    leaf = out.grad_fn.next_functions
+    assert leaf
+    done = len(launches)
+    with forward_ad.dual_level():
+        up = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            out.backward(up)
+    assert len(launches) == done
