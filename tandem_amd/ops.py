@@ -13,6 +13,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from ._lib import DISTILL_HOW, DTYPES as CODES, HEADS, POSITIONS, QK_SHAPE, check, lib, require_device_tensor
 
@@ -62,8 +63,24 @@ def _same_device(first, *others):
             raise ValueError(f"tensors on {first.device} and {t.device}")
 
 
+_PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
+_compiling, _tracing, _modes, _has_key = (torch.compiler.is_dynamo_compiling, torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack,
+                                          torch._C._dispatch_tls_is_dispatch_key_included)
+
+
+def _no_trace():
+    """Refuses a call that is being recorded: a launch leaves nothing in the record but the empty tensor that it fills. (A mode of any kind
+    shows on the stack or, before dispatch, as a key: asking which one costs a microsecond, and there hardly ever is one. torch.compile
+    leaves its graph for a launch, and doesn't need to be refused.)"""
+    if _compiling():
+        return
+    if _tracing() is not None or ((_modes() or _has_key(_PRE_DISPATCH)) and get_proxy_mode() is not None):
+        raise NotImplementedError("tandem_amd.ops can't be recorded by torch.jit.trace, make_fx or torch.export")
+
+
 def _call(t, entry, *args):
     """entry(*args, stream) on the current stream of `t`'s device: the launch goes to the current device, which may be another."""
+    _no_trace()
     device = t.get_device()
     if device == torch._C._cuda_getDevice():
         status = entry(*args, torch._C._cuda_getCurrentRawStream(device))

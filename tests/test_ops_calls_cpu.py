@@ -91,3 +91,38 @@ def test_an_upstream_gradient_with_a_tangent_is_refused(launches, name):
         with pytest.raises(NotImplementedError, match="forward mode"):
             out.backward(up)
     assert len(launches) == done
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_call_that_is_being_recorded_is_refused(launches, name):
+    """A trace would hold the result's memory without what is written there."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, given = operands()[name]
+    values = tuple(given.values())
+    for record in (lambda: torch.jit.trace(lambda *x: call(*x), values, check_trace=False), lambda: make_fx(lambda *x: call(*x))(*values),
+                   lambda: make_fx(lambda *x: call(*x), pre_dispatch=True)(*values)):
+        with pytest.raises(NotImplementedError, match="recorded"):
+            record()
+    assert not launches
+    call(**given)
+    assert launches
+
+
+def test_a_backward_pass_that_is_being_recorded_is_refused(launches):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, given = operands()["embedding"]
+    out = call(given["w"].requires_grad_())
+    with pytest.raises(NotImplementedError, match="recorded"):
+        make_fx(lambda g: torch.autograd.grad(out, given["w"], g, retain_graph=True))(torch.ones_like(out))
+    assert len(launches) == 1
+
+
+def test_a_compiled_program_leaves_its_graph_for_a_launch(launches):
+    call, given = operands()["embedding"]
+    w = given["w"].requires_grad_()
+    program = torch.compile(lambda w: call(w) * 0 + 2, backend="eager")
+    for n in (1, 2):
+        program(w).sum().backward()
+        assert [name for name, _ in launches] == ["tdm_k5_embedding", "tdm_k5_embedding_grad"] * n
