@@ -448,7 +448,7 @@ typedef struct tdm_distill_how {
 } tdm_distill_how;
 
 /* For a row x of logits [rows, vocab], the teacher's logits t [rows, k] at the columns teacher_index [rows, k], temperature T,
- * weight a and target y (targets [rows], NULL with weight 1: all rows count):
+ * weight a and target y (targets [rows]; NULL with weight 1: all rows count; without rows every operand may be NULL):
  *
  *     p = softmax(t / T),   row = a T^2 sum_k p_k (log p_k - log softmax(x / T)[index_k]) - (1 - a) log softmax(x)[y]
  *

@@ -832,7 +832,7 @@ int tdm_k7_distill(const tdm_distill_how* how, const void* logits, const void* t
   return guard([&] {
     check_how(how);
     const tdm_distill_how& h = *how;
-    require(h.weight == 1.0f || targets != nullptr, "distill: a weight below 1 needs targets");
+    require(h.rows == 0 || h.weight == 1.0f || targets != nullptr, "distill: a weight below 1 needs targets");
     require(loss != nullptr || grad != nullptr || h.rows == 0, "distill: neither loss nor gradient is wanted");
     require(h.rows == 0 || (logits != nullptr && ((teacher_index != nullptr && teacher_logits != nullptr) || h.weight == 0.0f)), "distill: null pointer");
     require(workspace != nullptr && workspace_bytes >= workspace_bytes_of(h) && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,

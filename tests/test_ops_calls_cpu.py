@@ -126,3 +126,17 @@ def test_a_compiled_program_leaves_its_graph_for_a_launch(launches):
     for n in (1, 2):
         program(w).sum().backward()
         assert [name for name, _ in launches] == ["tdm_k5_embedding", "tdm_k5_embedding_grad"] * n
+
+
+def test_an_empty_batch_with_hard_targets_is_no_error_in_the_library():
+    """No rows, so no targets either: an empty tensor's address is zero. Nothing is launched where no loss is wanted."""
+    from tandem_amd import _lib
+
+    L = _lib.lib()
+    work = torch.empty(4096, dtype=torch.uint8)
+    at = (work.data_ptr() + 15) // 16 * 16
+    for weight in (1.0, 0.5, 0.0):
+        for reduction in (0, 1, 2):
+            how = _lib.DISTILL_HOW.pack(0, 50, -100, 4, 0, 4, 0, 4, reduction, 1.0, weight, 1.0)
+            status = L.tdm_k7_distill(how, None, None, None, None, None, None, None, 0, at, L.tdm_k7_distill_workspace(how), None)
+            assert status == 0, (weight, reduction, L.tdm_last_error())
