@@ -556,9 +556,11 @@ class _Distill(torch.autograd.Function):
         _no_tangent(upstream)
         # the gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out
         # once; a second backward pass through the same graph computes its own.
+        # (Nor is it where hooks on saved tensors gave the logits back at another distance from a 16-byte boundary: the kernel takes both at one.)
+        logits, *operands = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
-        first = grad is not None
+        first = grad is not None and (grad.data_ptr() - logits.data_ptr()) % 16 == 0
         if not first:
-            grad = _empty_at_phase_of(ctx.saved_tensors[0])
-        _distill(*ctx.saved_tensors, ctx.how, ctx.each_row, False, grad, upstream if upstream.is_contiguous() else upstream.contiguous(), first, ctx.need)
+            grad = _empty_at_phase_of(logits)
+        _distill(logits, *operands, ctx.how, ctx.each_row, False, grad, upstream if upstream.is_contiguous() else upstream.contiguous(), first, ctx.need)
         return grad, None, None, None, None, None

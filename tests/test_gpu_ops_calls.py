@@ -24,3 +24,35 @@ def test_a_loss_of_no_rows_with_targets(dtype, weight, reduction):
     for got in (loss, alone, trained):
         assert got.shape == ((0,) if reduction == "none" else ()) and (got == 0).all()
     assert grad.shape == leaf.grad.shape == (0, 50)
+
+
+def distillation(rows, vocab, dtype, lead=0, seed=1):
+    """Logits that begin `lead` elements behind an allocation's start, a teacher's columns and logits, targets."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.zeros(lead + rows * vocab, device=DEV, dtype=dtype)[lead:].view(rows, vocab)
+    x.copy_(torch.randn(rows, vocab, generator=gen) * 2)
+    columns, t = torch.randint(0, vocab, (rows, 4), generator=gen).to(DEV), torch.randn(rows, 4, generator=gen).to(DEV)
+    return x, columns, t, torch.randint(0, vocab, (rows,), generator=gen).to(DEV)
+
+
+@pytest.mark.parametrize("lead", [0, 1, 3])
+@pytest.mark.parametrize("vocab", [251, 5003, 40001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_offloaded_logits_that_began_anywhere(dtype, vocab, lead):
+    """The copy that comes back begins on an allocation's boundary, the gradient that the forward pass left where the logits did."""
+    from tandem_amd import ops
+
+    x, columns, t, y = distillation(6, vocab, dtype, lead)
+    for up in (1.0, 0.5):
+        leaf = x.detach().requires_grad_()
+        assert leaf.data_ptr() == x.data_ptr()
+        with torch.autograd.graph.save_on_cpu():
+            loss = ops.distill_loss(leaf, columns, t, y, temperature=2.0, weight=0.5)
+        loss.backward(torch.tensor(up, device=DEV))
+        # a gradient that both times comes from the copy is the same bits; one from rows that begin elsewhere has its sums in another order: off by
+        # less than 2^-13 of a value each (4 R + V / 64 + 50 units of 2^-24, R < 16, V < 40002), and a step of the type where a rounding turns the other way
+        want = ops.distill_loss_and_grad(x.clone(), columns, t, y, temperature=2.0, weight=0.5, scale=up)[1]
+        if lead * x.element_size() % 16 == 0:
+            assert torch.equal(leaf.grad, want)
+        else:
+            assert leaf.grad.shape == want.shape and (leaf.grad.float() - want.float()).abs().max() <= (torch.finfo(dtype).eps + 2.0 ** -12) * want.float().abs().max()

@@ -140,3 +140,22 @@ def test_an_empty_batch_with_hard_targets_is_no_error_in_the_library():
             how = _lib.DISTILL_HOW.pack(0, 50, -100, 4, 0, 4, 0, 4, reduction, 1.0, weight, 1.0)
             status = L.tdm_k7_distill(how, None, None, None, None, None, None, None, 0, at, L.tdm_k7_distill_workspace(how), None)
             assert status == 0, (weight, reduction, L.tdm_last_error())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lead", [0, 1, 3])
+def test_logits_that_come_back_elsewhere_get_a_gradient_at_their_alignment(launches, dtype, lead):
+    """Hooks on saved tensors may give the backward pass a copy: the gradient that the forward pass left lies as the logits did then."""
+    from tandem_amd import ops
+
+    storage = torch.zeros(4 * 9 + 8, dtype=dtype)
+    x = storage[lead:lead + 36].view(4, 9).requires_grad_()
+    assert x.data_ptr() % 16 == lead * x.element_size() % 16  # torch's own allocations begin on 64 bytes
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.clone()):
+        loss = ops.distill_loss(x, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2))
+    for _ in range(2):
+        (grad,) = torch.autograd.grad(loss, x, retain_graph=True)
+        name, args = launches[-1]
+        logits, written, keep_ones = args[1], args[6], args[8]
+        assert name == "tdm_k7_distill" and logits % 16 == 0 and written == grad.data_ptr() and written % 16 == 0
+        assert grad.shape == x.shape and (lead == 0 or not keep_ones)
