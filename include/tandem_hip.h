@@ -70,6 +70,9 @@ int tdm_abi_version(void);
 /* Name, compute-unit count and memory of HIP device `device`. */
 int tdm_device_info(int device, char* name, int name_len, int* compute_units, int64_t* total_bytes);
 
+/* The number of the graph capture that `stream` is part of; 0: none, -1: failure. */
+int64_t tdm_stream_capture_id(tdm_stream stream);
+
 /* Launch geometry knob for measurements: workgroups per compute unit used by the
  * streaming kernels before their grids start to stride, 1..16384 (0 restores the built-in default, 16384: one
  * workgroup per tile up to 16 GiB per launch and stream on 256 compute units). Not needed for correctness; the
@@ -455,7 +458,8 @@ typedef struct tdm_distill_how {
  * loss (fp32: one value, or [rows] with TDM_DISTILL_NONE; NULL: not wanted) and grad [rows, vocab] (NULL: not wanted), the gradient
  * of scale * upstream * loss with respect to the logits, rounded once. upstream (fp32 in GPU memory: one value, or [rows]
  * with TDM_DISTILL_NONE) may be NULL: ones. With keep_ones the gradient of the rows whose upstream is 1 is left as it is: a caller that
- * has it from an earlier call computes only what an upstream value changes. A teacher's entry with a negative column or a logit of
+ * has it from an earlier call computes only what an upstream value changes. (In a graph that call belongs into the same graph: a replay
+ * finds what the last one's user made of the gradient.) A teacher's entry with a negative column or a logit of
  * -inf says nothing (the teacher's logits take no gradient); a row without another has no first term; entries of the same column add up. A column, or a target that
  * is used, outside the vocabulary and a NaN among the teacher's logits make the row's loss and gradient NaN; nothing is read there.
  * logits is contiguous; grad starts at the same distance from a 16-byte boundary as logits. The workspace starts

@@ -68,6 +68,7 @@ _SIGNATURES = {
     "tdm_abi_version": (ctypes.c_int, []),
     "tdm_device_info": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(ctypes.c_int),
                                        ctypes.POINTER(ctypes.c_int64)]),
+    "tdm_stream_capture_id": (ctypes.c_int64, [ctypes.c_void_p]),
     "tdm_set_blocks_per_cu": (ctypes.c_int, [ctypes.c_int]),
     "tdm_set_xcd_group": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
     "tdm_set_occupancy_pad": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),

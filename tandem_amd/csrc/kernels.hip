@@ -852,6 +852,20 @@ int tdm_build_geometry(int* k1_tile_bytes, int* workgroup_lanes, int* table_tile
   });
 }
 
+int64_t tdm_stream_capture_id(tdm_stream stream) {
+  int64_t id = -1;
+  guard([&] {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long number = 0;
+    const hipError_t err = hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &number);
+    if (err != hipSuccess) (void)hipGetLastError();  // a failed question is no failed launch
+    check_hip(err, "hipStreamGetCaptureInfo");
+    if (status == hipStreamCaptureStatusNone) id = 0;
+    if (status == hipStreamCaptureStatusActive) id = static_cast<int64_t>(number) + 1;
+  });
+  return id;
+}
+
 int tdm_set_blocks_per_cu(int blocks) {
   return guard([&] {
     if (blocks < 0 || blocks > kDefaultBlocksPerCu) throw Invalid("blocks per compute unit must be in [0, " + std::to_string(kDefaultBlocksPerCu) + "]");

@@ -541,25 +541,31 @@ def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, up
     return loss
 
 
+def _capture_of(t):
+    """The number of the graph capture that `t`'s current stream is part of (0: none, negative: unknown)."""
+    return lib().tdm_stream_capture_id(torch._C._cuda_getCurrentRawStream(t.get_device()))
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, targets, how, each_row):
         ctx.save_for_backward(logits, index, teacher, targets)
         ctx.how, ctx.each_row, ctx.need = how, each_row, lib().tdm_k7_distill_workspace(how)
         # float16 is trained with a scaled loss: a gradient computed here would be for nothing
-        ctx.grad = None if logits.dtype == torch.float16 else _empty_at_phase_of(logits)
+        ctx.grad, ctx.capture = (None, 0) if logits.dtype == torch.float16 else (_empty_at_phase_of(logits), _capture_of(logits))
         return _distill(logits, index, teacher, targets, how, each_row, True, ctx.grad, None, False, ctx.need)
 
     @staticmethod
     @_once
     def backward(ctx, upstream):
         _no_tangent(upstream)
-        # the gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out
-        # once; a second backward pass through the same graph computes its own.
-        # (Nor is it where hooks on saved tensors gave the logits back at another distance from a 16-byte boundary: the kernel takes both at one.)
+        # The gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out once; a second
+        # backward pass through the same graph computes its own. So does one whose logits hooks on saved tensors gave back at another distance from a
+        # 16-byte boundary (the kernel takes both at one), and one that is captured apart from its forward pass: replayed without it, it would
+        # hand out what the last replay's user made of the gradient.
         logits, *operands = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
-        first = grad is not None and (grad.data_ptr() - logits.data_ptr()) % 16 == 0
+        first = grad is not None and (grad.data_ptr() - logits.data_ptr()) % 16 == 0 and 0 <= ctx.capture == _capture_of(logits)
         if not first:
             grad = _empty_at_phase_of(logits)
         _distill(logits, *operands, ctx.how, ctx.each_row, False, grad, upstream if upstream.is_contiguous() else upstream.contiguous(), first, ctx.need)

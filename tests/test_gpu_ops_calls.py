@@ -56,3 +56,78 @@ def test_offloaded_logits_that_began_anywhere(dtype, vocab, lead):
             assert torch.equal(leaf.grad, want)
         else:
             assert leaf.grad.shape == want.shape and (leaf.grad.float() - want.float()).abs().max() <= (torch.finfo(dtype).eps + 2.0 ** -12) * want.float().abs().max()
+
+
+@pytest.mark.parametrize("forward_captured", [False, True])
+@pytest.mark.parametrize("vocab,dtype", [(256, torch.float32), (20000, torch.bfloat16)])
+def test_a_graph_that_holds_the_backward_pass_alone(vocab, dtype, forward_captured):
+    """Replayed without the forward pass, which ran eagerly or is a graph of its own, after the gradient that the last replay gave was changed."""
+    from tandem_amd import ops
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):  # everything on one stream, the leaf's first use too
+        x, columns, t, y = distillation(70, vocab, dtype)
+        leaf = x.clone().requires_grad_()
+        loss_of = lambda: ops.distill_loss(leaf, columns, t, y, temperature=2.0, weight=0.5)  # noqa: E731
+        want = torch.autograd.grad(loss_of(), leaf)[0]
+        torch.cuda.synchronize()
+        fore, back = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        if forward_captured:
+            with torch.cuda.graph(fore, stream=s):
+                loss = loss_of()
+        else:
+            loss = loss_of()
+        with torch.cuda.graph(back, stream=s, **({"pool": fore.pool()} if forward_captured else {})):
+            (grad,) = torch.autograd.grad(loss, leaf)
+        if forward_captured:
+            fore.replay()
+        for _ in range(3):
+            back.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(grad, want)
+            grad.mul_(3.0)
+            torch.cuda.synchronize()
+
+
+def test_a_captured_step_hands_out_its_own_forward_pass_s_gradient():
+    """Within one capture the number is the same on both threads, and the gradient is computed once."""
+    from tandem_amd import _lib, ops
+
+    x, columns, t, y = distillation(70, 20000, torch.bfloat16)
+    leaf, ids = x.clone().requires_grad_(), []
+    number = lambda: ids.append(_lib.lib().tdm_stream_capture_id(torch.cuda.current_stream().cuda_stream))  # noqa: E731
+
+    class Note(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, z):
+            number()
+            return z.view_as(z)
+
+        @staticmethod
+        def backward(ctx, g):
+            number()
+            return g
+
+    def step():
+        loss = ops.distill_loss(Note.apply(leaf), columns, t, y, temperature=2.0, weight=0.5)
+        return loss, *torch.autograd.grad(loss, leaf)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step())
+    assert ids[:2] == [0, 0] and 0 < ids[2] == ids[3] and 0 < ids[4] == ids[5] != ids[2]
+    for _ in range(2):
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+            out[1].zero_()
+            torch.cuda.synchronize()

@@ -9,7 +9,10 @@ class NoLaunches:
     """The library, its kernels left out: every launch is noted with its arguments."""
 
     def __init__(self, library):
-        self.library, self.calls = library, []
+        self.library, self.calls, self.capture = library, [], 0
+
+    def tdm_stream_capture_id(self, stream):
+        return self.capture
 
     def __getattr__(self, name):
         if not name.startswith("tdm_k") or name.endswith("_workspace"):
@@ -33,6 +36,13 @@ def launches(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)  # a CPU tensor's get_device()
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
     return stand_in.calls
+
+
+@pytest.fixture
+def stand_in(launches):
+    from tandem_amd import ops
+
+    return ops.lib()
 
 
 def operands():
@@ -159,3 +169,19 @@ def test_logits_that_come_back_elsewhere_get_a_gradient_at_their_alignment(launc
         logits, written, keep_ones = args[1], args[6], args[8]
         assert name == "tdm_k7_distill" and logits % 16 == 0 and written == grad.data_ptr() and written % 16 == 0
         assert grad.shape == x.shape and (lead == 0 or not keep_ones)
+
+
+@pytest.mark.parametrize("forward,backward,handed_out", [(0, 0, True), (7, 7, True), (0, 7, False), (7, 0, False), (7, 8, False), (-1, -1, False)])
+def test_the_forward_pass_s_gradient_stays_within_its_capture(stand_in, forward, backward, handed_out):
+    """A graph that holds the backward pass alone is replayed without the forward pass: a gradient handed out there would be what the last
+    replay's user made of it. The forward pass's is handed out within one capture, or where there is none."""
+    from tandem_amd import ops
+
+    x = torch.zeros(4, 12, requires_grad=True)
+    stand_in.capture = forward
+    loss = ops.distill_loss(x, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2))
+    left = stand_in.calls[-1][1][6]
+    stand_in.capture = backward
+    (grad,) = torch.autograd.grad(loss, x)
+    _, args = stand_in.calls[-1]
+    assert args[8] == handed_out and args[6] == grad.data_ptr() and (args[6] == left) == handed_out
