@@ -111,7 +111,7 @@ def test_a_captured_step_hands_out_its_own_forward_pass_s_gradient():
 
     def step():
         loss = ops.distill_loss(Note.apply(leaf), columns, t, y, temperature=2.0, weight=0.5)
-        return loss, *torch.autograd.grad(loss, leaf)
+        return loss.detach(), *torch.autograd.grad(loss, leaf)  # no graph of the leaf's outlives the step
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
