@@ -217,7 +217,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
 
     q and k may be views of any strides whose last dimension is contiguous; float32, float16 or bfloat16, the weights of the
     same dtype or float32. positions: int64 or int32, of a shape that expands to [batch, tokens]; inv_freq: float64
-    (rope_frequencies). Angles are computed in float64, so far positions keep their precision. Single tokens are a
+    (rope_frequencies), it takes no gradient. Angles are computed in float64, so far positions keep their precision. Single tokens are a
     batch of one token each."""
     x = _separate(q, k)
     how = _check_qk(x, q, q_weight, k_weight, positions, inv_freq, eps, interleaved)
@@ -353,6 +353,8 @@ def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved
         raise ValueError("positions: an int64 or int32 tensor")
     require_device_tensor(inv_freq, "qk_norm_rope(inv_freq)")
     _no_tangent(inv_freq)
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise ValueError("inv_freq takes no gradient")
     rotary = 2 * inv_freq.numel()
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or rotary > x.dim:
         raise ValueError(f"inv_freq: at most {x.dim // 2} float64 values")

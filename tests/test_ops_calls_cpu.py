@@ -185,3 +185,14 @@ def test_the_forward_pass_s_gradient_stays_within_its_capture(stand_in, forward,
     (grad,) = torch.autograd.grad(loss, x)
     _, args = stand_in.calls[-1]
     assert args[8] == handed_out and args[6] == grad.data_ptr() and (args[6] == left) == handed_out
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "qkv_norm_rope"])
+def test_frequencies_that_want_a_gradient_are_refused(launches, name):
+    """They get none: a trained table of angles would stay as it is without a word."""
+    call, given = operands()[name]
+    with pytest.raises(ValueError, match="inv_freq"):
+        call(**{**given, "freq": given["freq"].clone().requires_grad_()})
+    with torch.no_grad():
+        call(**{**given, "freq": given["freq"].clone().requires_grad_()})
+    assert len(launches) == 1
