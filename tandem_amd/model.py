@@ -74,6 +74,8 @@ class Attention(nn.Module):
     def forward(self, x):
         batch, steps, width = x.shape
         if self.rotary:
+            if steps > self._seq:  # a single position would be repeated instead
+                raise ValueError(f"{steps} tokens for a model of {self._seq} positions")
             positions, inv_freq = self._rotation(x.device)
             heads = ops.qkv_norm_rope(self.qkv(x), self.heads, self.heads, self.q_norm, self.k_norm, positions[:steps], inv_freq)
             mixed = F.scaled_dot_product_attention(*(part.transpose(1, 2) for part in heads), is_causal=True)

@@ -196,3 +196,14 @@ def test_frequencies_that_want_a_gradient_are_refused(launches, name):
     with torch.no_grad():
         call(**{**given, "freq": given["freq"].clone().requires_grad_()})
     assert len(launches) == 1
+
+
+def test_the_rotary_model_refuses_sequences_beyond_its_length(launches):
+    """Also of a model for one position, whose position would be repeated."""
+    from tandem_amd.model import GPT, Config
+
+    for seq in (1, 4):
+        model = GPT(Config(seq=seq, layers=1, heads=2, dim=16, rotary=True))
+        model(torch.zeros(1, seq, dtype=torch.int64))
+        with pytest.raises(ValueError, match=f"{seq + 1} tokens"):
+            model(torch.zeros(1, seq + 1, dtype=torch.int64))
