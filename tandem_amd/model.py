@@ -101,16 +101,26 @@ class Block(nn.Module):
         return x + self.out(F.gelu(self.fc(self.ln2(x))))
 
 
+class ScaledEmbedding(nn.Embedding):
+    """torch's embedding in everything but its pass: scale * weight[idx] by ops.embedding."""
+
+    def __init__(self, vocab, dim, scale):
+        super().__init__(vocab, dim)
+        self.scale = scale
+
+    def forward(self, idx):
+        return ops.embedding(idx, self.weight, scale=self.scale, padding_idx=self.padding_idx)
+
+
 class Embed(nn.Module):
     def __init__(self, cfg):
         super().__init__()
-        self.tok = nn.Embedding(cfg.vocab, cfg.dim)
-        self.scale = cfg.embed_scale
+        self.tok = ScaledEmbedding(cfg.vocab, cfg.dim, cfg.embed_scale) if cfg.rotary else nn.Embedding(cfg.vocab, cfg.dim)
         self.pos = None if cfg.rotary else nn.Embedding(cfg.seq, cfg.dim)
 
     def forward(self, idx):
         if self.pos is None:
-            return ops.embedding(idx, self.tok.weight, scale=self.scale)
+            return self.tok(idx)
         where = torch.arange(idx.shape[1], device=idx.device)
         return self.tok(idx) + self.pos(where)
 

@@ -207,3 +207,24 @@ def test_the_rotary_model_refuses_sequences_beyond_its_length(launches):
         model(torch.zeros(1, seq, dtype=torch.int64))
         with pytest.raises(ValueError, match=f"{seq + 1} tokens"):
             model(torch.zeros(1, seq + 1, dtype=torch.int64))
+
+
+def test_hooks_on_the_rotary_model_s_token_embedding_run(launches):
+    """The embedding is a module of its own, as in the plain model: what is registered on it is called, and what it is replaced by is used."""
+    from tandem_amd.model import GPT, Config
+
+    for rotary in (False, True):
+        model = GPT(Config(seq=8, layers=1, heads=2, dim=16, rotary=rotary, embed_scale=3.0 if rotary else 1.0))
+        seen = []
+        model.embed.tok.register_forward_pre_hook(lambda module, args: seen.append(args[0].shape))
+        model.embed.tok.register_forward_hook(lambda module, args, out: seen.append(out.shape))
+        model(torch.zeros(2, 5, dtype=torch.int64))
+        assert seen == [(2, 5), (2, 5, 16)], rotary
+        assert isinstance(model.embed.tok, torch.nn.Embedding) and "embed.tok.weight" in model.state_dict()
+        model.embed.tok = torch.nn.Identity()
+        model.embed.tok.forward = lambda idx: torch.ones(*idx.shape, 16)
+        done = [name for name, _ in launches].count("tdm_k5_embedding")
+        model(torch.zeros(2, 5, dtype=torch.int64))
+        assert [name for name, _ in launches].count("tdm_k5_embedding") == done
+    name, args = next(call for call in launches if call[0] == "tdm_k5_embedding")
+    assert args[-2] == 3.0
