@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
   if constexpr (kHeld > 0) {
     from = stretch(row_at(row) + body.head, body.vecs * 16);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = load16<kStream>(from, lane16, i * kG * 16);
+    for (int i = 0; i < kHeld; ++i) held[i] = load16(from, lane16, i * kG * 16);
   }
   if (a.counts) {
     const float n = counted_by_wave<kG>(a);
@@ -431,9 +431,9 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
           }
           Vec16 out = pack16<T>(f);
           if constexpr (sizeof(T) == 2 && kApart) out ^= sign;
-          store16<kStream>(out, to, lane16, i * kG * 16);
+          store16(out, to, lane16, i * kG * 16);
         }
-        if (i < kEarly) held[i] = load16<kStream>(from, lane16, i * kG * 16);
+        if (i < kEarly) held[i] = load16(from, lane16, i * kG * 16);
         __builtin_amdgcn_sched_barrier(0);  // one vector at a time: interleaved, they take twice the registers
       }
     }
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_t
     __syncthreads();
     if constexpr (kHeld > 0) {
 #pragma unroll
-      for (int i = kEarly; i < kHeld; ++i) held[i] = load16<kStream>(from, lane16, i * kG * 16);
+      for (int i = kEarly; i < kHeld; ++i) held[i] = load16(from, lane16, i * kG * 16);
     }
     if (a.rows_loss != nullptr && tid == 0) {
       float loss = wrong;

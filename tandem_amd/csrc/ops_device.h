@@ -35,7 +35,6 @@ struct Pack {
   using raw_t = typename RawOf<kN * static_cast<int>(sizeof(T))>::type;
   raw_t raw;
   static __device__ __forceinline__ Pack load(const T* at) { return Pack{*reinterpret_cast<const raw_t*>(at)}; }
-  static __device__ __forceinline__ Pack load_nt(const T* at) { return Pack{__builtin_nontemporal_load(reinterpret_cast<const raw_t*>(at))}; }
   __device__ __forceinline__ void store(T* at) const { *reinterpret_cast<raw_t*>(at) = raw; }
   __device__ __forceinline__ void store_nt(T* at) const { __builtin_nontemporal_store(raw, reinterpret_cast<raw_t*>(at)); }
 
@@ -106,14 +105,12 @@ __device__ __forceinline__ Stretch stretch(const void* base, int bytes) { return
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t behind(const Stretch& s, int offset) {
   return __builtin_amdgcn_make_buffer_rsrc(s.base + offset, 0, std::max(s.bytes - offset, 0), 0x00027000);  // raw, 32-bit elements
 }
-constexpr int kPlain = 0, kStream = 2;  // cache policies: cached; non-temporal
-template <int kPolicy>
+constexpr int kStream = 2;  // the accesses' cache policy: non-temporal
 __device__ __forceinline__ Vec16 load16(const Stretch& from, int lane_offset, int offset) {
-  return __builtin_amdgcn_raw_buffer_load_b128(behind(from, offset), lane_offset, 0, kPolicy);
+  return __builtin_amdgcn_raw_buffer_load_b128(behind(from, offset), lane_offset, 0, kStream);
 }
-template <int kPolicy>
 __device__ __forceinline__ void store16(const Vec16& v, const Stretch& to, int lane_offset, int offset) {
-  __builtin_amdgcn_raw_buffer_store_b128(v, behind(to, offset), lane_offset, 0, kPolicy);
+  __builtin_amdgcn_raw_buffer_store_b128(v, behind(to, offset), lane_offset, 0, kStream);
 }
 
 // Reductions over the 64 lanes of a wave by DPP: sums along the rows of 16 lanes, then rows 0 and 2 into 1 and 3, then the lower

@@ -18,7 +18,7 @@ using namespace tandem_hip::ops;
 extern "C" __global__ void copy(const void* from, void* to, int bytes) {{
   const auto a = stretch(from, bytes), b = stretch(to, bytes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) store16<kStream>(load16<kStream>(a, threadIdx.x * 16, i * 16384), b, threadIdx.x * 16, i * 16384);
+  for (int i = 0; i < 4; ++i) store16(load16(a, threadIdx.x * 16, i * 16384), b, threadIdx.x * 16, i * 16384);
 }}
 ''')
     out = tmp_path / "stretch.s"
