@@ -27,9 +27,8 @@ def _on_gpu(t, what):
 
 
 def _no_tangent(*tensors):
-    """Refuses operands that carry a tangent of forward-mode differentiation: the kernels would drop it, and the result's derivative be zero."""
-    if forward_ad._current_level < 0:  # no level is open: no tensor has one
-        return
+    """Refuses operands that carry a tangent of forward-mode differentiation: the kernels would drop it, and the result's derivative be zero.
+    For where a level is open (forward_ad._current_level >= 0): no tensor has one otherwise."""
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError("tandem_amd.ops has no derivatives in forward mode")
@@ -39,11 +38,16 @@ def _tensor(t, what):
     _on_gpu(t, what)
     if t.dtype not in DTYPES:
         raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
-    _no_tangent(t)
+    if forward_ad._current_level >= 0:
+        _no_tangent(t)
 
 
 def _floating(t, what):
-    _tensor(t, what)
+    _on_gpu(t, what)
+    if t.dtype not in DTYPES:
+        raise ValueError(f"{what}: float32, float16 or bfloat16, not {t.dtype}")
+    if forward_ad._current_level >= 0:
+        _no_tangent(t)
     if not t.is_contiguous():
         raise ValueError(f"{what}: needs a contiguous tensor")
 
@@ -63,30 +67,30 @@ def _same_device(first, *others):
             raise ValueError(f"tensors on {first.device} and {t.device}")
 
 
+# A call's own queries of torch, bound once: they are most of what a small call costs the host.
 _PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
 _compiling, _tracing, _modes, _has_key = (torch.compiler.is_dynamo_compiling, torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack,
                                           torch._C._dispatch_tls_is_dispatch_key_included)
+_current_device, _current_stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))  # None: torch without a GPU
 
 
-def _no_trace():
-    """Refuses a call that is being recorded: a launch leaves nothing in the record but the empty tensor that it fills. (A mode of any kind
-    shows on the stack or, before dispatch, as a key: asking which one costs a microsecond, and there hardly ever is one. torch.compile
-    leaves its graph for a launch, and doesn't need to be refused.)"""
-    if _compiling():
-        return
-    if _tracing() is not None or ((_modes() or _has_key(_PRE_DISPATCH)) and get_proxy_mode() is not None):
-        raise NotImplementedError("tandem_amd.ops can't be recorded by torch.jit.trace, make_fx or torch.export")
+def _recorded():
+    """Whether a trace is being made: a launch leaves nothing in it but the empty tensor that it fills. (torch.compile leaves its graph for
+    a launch, and is no such trace.)"""
+    return _tracing() is not None or get_proxy_mode() is not None
 
 
 def _call(t, entry, *args):
     """entry(*args, stream) on the current stream of `t`'s device: the launch goes to the current device, which may be another."""
-    _no_trace()
+    # a mode of any kind shows on the stack or, before dispatch, as a key; asking which one takes longer, and there hardly ever is one
+    if not _compiling() and (_tracing() is not None or _modes() or _has_key(_PRE_DISPATCH)) and _recorded():
+        raise NotImplementedError("tandem_amd.ops can't be recorded by torch.jit.trace, make_fx or torch.export")
     device = t.get_device()
-    if device == torch._C._cuda_getDevice():
-        status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+    if device == _current_device():
+        status = entry(*args, _current_stream(device))
     else:
         with torch.cuda.device(device):
-            status = entry(*args, torch._C._cuda_getCurrentRawStream(device))
+            status = entry(*args, _current_stream(device))
     if status:
         check(status)
 
@@ -141,7 +145,8 @@ def _check_embedding(tokens, weight, padding_idx):
 
 def _embedding(tokens, weight, scale):
     tokens = _indices(tokens, "embedding(tokens)")
-    _same_device(weight, tokens)
+    if tokens.get_device() != weight.get_device():
+        _same_device(weight, tokens)
     vocab, dim = weight.shape
     out = weight.new_empty((*tokens.shape, dim))
     _call(weight, lib().tdm_k5_embedding, weight.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), tokens.numel(), vocab, dim,
@@ -170,7 +175,8 @@ def _embedding_grad(grad, tokens, vocab, scale, padding):
 
 
 def _embedding_backward(grad, tokens, vocab, dim, scale, padding, need):
-    _no_tangent(grad)
+    if forward_ad._current_level >= 0:
+        _no_tangent(grad)
     out = grad.new_empty((vocab, dim))
     work = _workspace(need, grad)
     _call(grad, lib().tdm_k5_embedding_grad, grad.data_ptr(), tokens.data_ptr(), CODES[tokens.dtype], out.data_ptr(), _ptr(work), need,
@@ -352,7 +358,8 @@ def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved
     if not isinstance(positions, torch.Tensor) or positions.dtype not in INDEX_DTYPES:
         raise ValueError("positions: an int64 or int32 tensor")
     require_device_tensor(inv_freq, "qk_norm_rope(inv_freq)")
-    _no_tangent(inv_freq)
+    if forward_ad._current_level >= 0:
+        _no_tangent(inv_freq)
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise ValueError("inv_freq takes no gradient")
     rotary = 2 * inv_freq.numel()
@@ -401,7 +408,8 @@ def _qk_need(how):
 
 
 def _qk_backward(dq_out, dk_out, dv_out, like, q_weight, k_weight, x, how, dx, need):
-    _no_tangent(dq_out, dk_out, dv_out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(dq_out, dk_out, dv_out)
     dq_out, dk_out, dv_out = _rows(dq_out), _rows(dk_out), _rows(dv_out)
     work = _workspace(need, like)
     dqw, dkw = None if q_weight is None else torch.empty_like(q_weight), None if k_weight is None else torch.empty_like(k_weight)
@@ -545,7 +553,7 @@ def _distill(logits, index, teacher, targets, how, each_row, want_loss, grad, up
 
 def _capture_of(t):
     """The number of the graph capture that `t`'s current stream is part of (0: none, negative: unknown)."""
-    return lib().tdm_stream_capture_id(torch._C._cuda_getCurrentRawStream(t.get_device()))
+    return lib().tdm_stream_capture_id(_current_stream(t.get_device()))
 
 
 class _Distill(torch.autograd.Function):
@@ -560,7 +568,8 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, upstream):
-        _no_tangent(upstream)
+        if forward_ad._current_level >= 0:
+            _no_tangent(upstream)
         # The gradient for an upstream of one is there: the kernel leaves the rows alone for which it is one. It is handed out once; a second
         # backward pass through the same graph computes its own. So does one whose logits hooks on saved tensors gave back at another distance from a
         # 16-byte boundary (the kernel takes both at one), and one that is captured apart from its forward pass: replayed without it, it would

@@ -33,8 +33,8 @@ def launches(monkeypatch):
     monkeypatch.setattr(ops, "lib", lambda: stand_in)
     monkeypatch.setattr(ops, "_on_gpu", lambda t, what: None)
     monkeypatch.setattr(ops, "require_device_tensor", lambda t, what: None)
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)  # a CPU tensor's get_device()
-    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
+    monkeypatch.setattr(ops, "_current_device", lambda: -1)  # a CPU tensor's get_device()
+    monkeypatch.setattr(ops, "_current_stream", lambda device: 0)
     return stand_in.calls
 
 
