@@ -95,6 +95,17 @@ def _call(t, entry, *args):
         check(status)
 
 
+def _ptr(t):
+    """The address of an operand that may be missing. One whose storage has been given back (a sharded weight's between its uses) has the address
+    zero, which says "missing" to the library; so has an empty one, which may be."""
+    if t is None:
+        return None
+    at = t.data_ptr()
+    if at == 0 and t.numel() > 0:
+        raise ValueError(f"an operand of {list(t.shape)} has no memory")
+    return at
+
+
 def _workspace(bytes_needed, like):
     if bytes_needed < 0:
         raise ValueError(lib().tdm_last_error().decode(errors="replace"))
@@ -321,7 +332,7 @@ def _view(t):
     if t is None:
         return HEADS.pack(0, 0, 0, 0)
     strides = t.stride()
-    return HEADS.pack(t.data_ptr(), *strides[:-1]) if len(strides) == 4 else HEADS.pack(t.data_ptr(), 0, *strides[:-1])
+    return HEADS.pack(_ptr(t), *strides[:-1]) if len(strides) == 4 else HEADS.pack(_ptr(t), 0, *strides[:-1])
 
 
 def _wants_grad(w):
@@ -380,10 +391,6 @@ def _check_qk(x, like, q_weight, k_weight, positions, inv_freq, eps, interleaved
     except struct.error as e:
         raise ValueError(f"qk_norm_rope: {e}") from None
     return how
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _qk_forward(like, q_weight, k_weight, x, how):

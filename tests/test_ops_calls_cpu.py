@@ -228,3 +228,33 @@ def test_hooks_on_the_rotary_model_s_token_embedding_run(launches):
         assert [name for name, _ in launches].count("tdm_k5_embedding") == done
     name, args = next(call for call in launches if call[0] == "tdm_k5_embedding")
     assert args[-2] == 3.0
+
+
+def without_memory(t):
+    """A tensor of t's shape whose storage has been given back, as sharded weights between their uses: its address is zero."""
+    t = t.clone()
+    t.untyped_storage().resize_(0)
+    assert t.data_ptr() == 0
+    return t
+
+
+@pytest.mark.parametrize("name,which", [(name, which) for name in ("qk_norm_rope", "qk_norm_rope_grad", "qkv_norm_rope", "qkv_norm_rope_grad")
+                                        for which in ("qw", "kw", "dq", "dk", "dv") if which in ("qw", "kw") or (name.endswith("grad") and (which != "dv" or "qkv" in name))])
+def test_an_operand_without_memory_is_no_missing_operand(launches, name, which):
+    """For the library an address of zero is "none": weights of one, upstream gradients of zero. (It refuses it itself where an operand is needed.)"""
+    call, given = operands()[name]
+    operand = without_memory(given[which])
+    with pytest.raises(ValueError, match="memory"):
+        call(**{**given, which: operand})
+    assert not launches
+
+
+def test_targets_and_upstream_gradients_without_memory_are_refused(launches):
+    from tandem_amd import ops
+
+    x, columns, t, y = torch.randn(3, 9, requires_grad=True), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2), torch.tensor([1, 2, 3])
+    with pytest.raises(ValueError, match="memory"):
+        ops.distill_loss(x, columns, t, targets=without_memory(y))
+    loss = ops.distill_loss(x, columns, t, targets=y, reduction="none")
+    with pytest.raises(ValueError, match="memory"):
+        loss.backward(without_memory(torch.ones(3)))
