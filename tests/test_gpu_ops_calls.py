@@ -131,3 +131,66 @@ def test_a_captured_step_hands_out_its_own_forward_pass_s_gradient():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
             out[1].zero_()
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("batch,tokens,hq,hk,d,rotary,dtype", [(2, 5, 3, 1, 64, 64, torch.bfloat16), (3, 67, 5, 5, 80, 40, torch.float32), (1, 1, 9, 2, 128, 128, torch.float16),
+                                                               (2, 1000, 12, 4, 2, 2, torch.bfloat16), (1, 300, 1, 1, 510, 10, torch.float16)])
+def test_heads_that_lie_apart_leave_what_is_between_them(batch, tokens, hq, hk, d, rotary, dtype, interleaved):
+    """Results written into the middle of larger heads, tokens and batches: everything around them stays, and they are those of the plain call."""
+    from tandem_amd import _lib, ops
+
+    gen = torch.Generator().manual_seed(9)
+    q, k = (torch.randn(batch, tokens, h, d, generator=gen).to(dtype).to(DEV) for h in (hq, hk))
+    up = [torch.randn(t.shape, generator=gen).to(dtype).to(DEV) for t in (q, k, k)]
+    qw, kw = (torch.randn(d, generator=gen).to(DEV) for _ in range(2))
+    pos, freq = torch.arange(tokens, device=DEV) + 7, ops.rope_frequencies(rotary)
+    code = ops.CODES[dtype]
+    shape, at = _lib.QK_SHAPE.pack(batch, tokens, hq, hk, d, rotary, interleaved, code, 0, 4, 1e-6), _lib.POSITIONS.pack(pos.data_ptr(), 0, 1)
+    heads = lambda x: _lib.HEADS.pack(x.data_ptr(), *x.stride()[:3])  # noqa: E731
+    stream = torch.cuda.current_stream().cuda_stream
+    L = _lib.lib()
+
+    def roomy(t):
+        around = torch.full((t.shape[0] + 1, t.shape[1] + 2, t.shape[2] + 1, d + 6), 7.0, dtype=dtype, device=DEV)
+        return around, around[:t.shape[0], 1:-1, :t.shape[2], 2:2 + d]
+
+    def untouched(around, inside):
+        inside.fill_(7.0)
+        return bool((around == 7.0).all())
+
+    (qa, qo), (ka, ko) = roomy(q), roomy(k)
+    _lib.check(L.tdm_k6_qk_norm_rope(shape, heads(q), heads(k), qw.data_ptr(), kw.data_ptr(), at, freq.data_ptr(), heads(qo), heads(ko), stream))
+    want = ops.qk_norm_rope(q, k, qw, kw, pos, freq, interleaved=bool(interleaved))
+    # another width of access, so other lanes hold a head: its sum has another order, off by up to d 2^-24 of it, and a rounding may turn the other way
+    near = lambda a, b: torch.isfinite(a).all() and ((a.float() - b.float()).abs() <= (torch.finfo(dtype).eps + 2.0 ** -13) * b.float().abs().amax(-1, True)).all()  # noqa: E731
+    assert near(qo, want[0]) and near(ko, want[1])
+    assert untouched(qa, qo) and untouched(ka, ko)
+    (dqa, dq), (dka, dk), (dva, dv) = roomy(q), roomy(k), roomy(k)
+    need = L.tdm_k6_qk_norm_rope_grad_workspace(shape)
+    work = torch.full((need + 64,), 0xFF, dtype=torch.uint8, device=DEV)
+    dw = torch.full((2, d + 2), 7.0, device=DEV)
+    _lib.check(L.tdm_k6_qk_norm_rope_grad(shape, heads(up[0]), heads(up[1]), heads(up[2]), heads(q), heads(k), qw.data_ptr(), kw.data_ptr(), at, freq.data_ptr(),
+                                          heads(dq), heads(dk), heads(dv), dw[0, 1:].data_ptr(), dw[1, 1:].data_ptr(), work.data_ptr(), need, stream))
+    want = ops.qk_norm_rope_grad(up[0], up[1], q, k, qw, kw, pos, freq, interleaved=bool(interleaved))
+    assert near(dq, want[0]) and near(dk, want[1]) and torch.equal(dv, up[2])
+    for got, ref, x, g in zip(dw[:, 1:-1], want[2:], (q, k), up):
+        # N terms in two orders, each of at most sqrt(2) times its row's largest upstream value times the normed element; no term passes N additions
+        x, terms = x.double(), x[..., 0].numel()
+        most = (2 ** 0.5 * g.double().abs().amax(-1, True) * (x * x.square().mean(-1, True).rsqrt()).abs()).sum((0, 1, 2))
+        assert ((got - ref).abs() <= 2 * (terms + 16) * 2.0 ** -24 * most).all()
+    assert (dw[:, 0] == 7).all() and (dw[:, -1] == 7).all() and (work[need:] == 0xFF).all()
+    assert untouched(dqa, dq) and untouched(dka, dk) and untouched(dva, dv)
+
+
+@pytest.mark.parametrize("vocab,dim,n,dtype,lead", [(50, 999, 37, torch.float16, 1), (50, 64, 1, torch.bfloat16, 0), (7, 3, 1030, torch.float32, 3), (9, 2050, 5, torch.bfloat16, 2)])
+def test_a_lookup_writes_its_rows_and_nothing_else(vocab, dim, n, dtype, lead):
+    from tandem_amd import _lib, ops
+
+    gen = torch.Generator().manual_seed(10)
+    w, tokens = torch.randn(vocab, dim, generator=gen).to(dtype).to(DEV), torch.randint(0, vocab, (n,), generator=gen).to(DEV)
+    around = torch.full((64 + lead + n * dim + 64,), 7.0, dtype=dtype, device=DEV)
+    out = around[64 + lead:64 + lead + n * dim]
+    _lib.check(_lib.lib().tdm_k5_embedding(w.data_ptr(), tokens.data_ptr(), 4, out.data_ptr(), n, vocab, dim, ops.CODES[dtype], 1.0, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out.view(n, dim), w[tokens])
+    assert (around[:64 + lead] == 7).all() and (around[64 + lead + n * dim:] == 7).all()
