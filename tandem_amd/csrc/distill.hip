@@ -74,8 +74,8 @@ __device__ __forceinline__ Body body_of(const T* x, int64_t vocab) {
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
 // What the two temperatures, T and 1, need of d = x - m: kOne exponential where one of them does for both parts (a = 0, a = 1 or T = 1);
-// kTwo; or one again, F, of which both are powers, for the usual T = 2 (F, F^2) and T = 1.5 (F^2, F^3): 1031 rows of 50021 fp16
-// logits take 56 us instead of 64, 4096 rows 196 and 201 instead of 212.
+// kTwo; or one again, F, of which both are powers, for T = 2 (F, F^2) and T = 1.5 (F^2, F^3): 1031 rows of 50021 fp16
+// logits take 57 us instead of 64, 4096 rows 196 and 201 instead of 212. Every other temperature takes two.
 enum Mix { kOne, kTwo, kSquare, kCube };
 Mix mix_of(float weight, float temperature) {
   if (weight <= 0.0f || weight >= 1.0f || temperature == 1.0f) return kOne;
@@ -176,7 +176,7 @@ constexpr uint32_t kNoColumn = 0xffffffffu;
 // its vectors makes room for the next row's: loads, exponentials and stores are under way at the same time with one workgroup per
 // compute unit. The teacher's entries are one lane's each (k <= kG): their elements and the target's are written again after the row, behind
 // a second barrier. Columns named twice are found by a hash table in LDS, and only then summed over all entries. 8192 rows of 131072 bf16
-// logits and their gradient take 806 us, 5.3 TB/s: bound by memory, reads and writes mixed (797 us with the exponentials taken out).
+// logits and their gradient take 809 us, 5.3 TB/s: bound by memory, reads and writes mixed (797 us with the exponentials taken out).
 template <typename T, int kG, int kHeld, Mix kMix>
 __global__ __launch_bounds__(kG, 4) void distill_kernel(DistillArgs a, int log_table) {
   constexpr int kN = per_vec<T>(), kWaves = kG / kWave;

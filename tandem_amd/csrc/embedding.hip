@@ -512,7 +512,7 @@ __device__ void zero_rows(const SumArgs& a) {
 
 // Bound by memory where the table is large: 32768 rows of 2048 bf16 into 131072, 134 MB read and 439 MB written here, take 103 us, 5.6 TB/s.
 // Eight rows of g are under way per wave. Chunks of equal length, not one token's rows each: byte tokens, some of which come
-// hundreds of times, keep every wave busy (8192 x 512 fp32 for 256 tokens: 6.8 us for 17 MB, and 4.7 for the join).
+// hundreds of times, keep every wave busy (8192 x 768 fp32 for 256 tokens: 6.5 us for 25 MB, and 4.8 for the join).
 template <typename T, int kBytes>
 __global__ __launch_bounds__(kSumThreads) void embedding_sum_kernel(SumArgs a) {
   constexpr int kN = kBytes / static_cast<int>(sizeof(T));
@@ -744,10 +744,11 @@ __global__ __launch_bounds__(kRowThreads) void embedding_row_kernel(RowArgs a) {
 
 constexpr int64_t kMostTokens = int64_t(1) << 28;  // the sums' launch stays below 2^32 lanes
 
-// Whether a gradient is the one launch's: at most 1024 workgroups, a row's 512 bytes each.
+// Whether a gradient is the one launch's: at most 1024 workgroups, a row's 512 bytes each, and 4096 tokens whatever the accesses' width (8192 would
+// pay with wide loads only, see the kernel).
 bool one_launch(int64_t n, int64_t vocab, int64_t dim, int es) { return n <= kRowTokens && vocab * ((dim * es + 511) / 512) <= 1024; }
 
-constexpr int64_t kMostVocab = int64_t(1) << 24;  // 2^14 workgroups place the tokens
+constexpr int64_t kMostVocab = int64_t(1) << 24;  // 2^15 workgroups place the tokens
 
 // Entries of a chunk: 64, or fewer as long as there are fewer than 2048 waves of 512 columns.
 int chunk_of(int64_t n, int64_t dim) {
@@ -806,7 +807,8 @@ Workspace workspace_of(int64_t n, int64_t vocab, int64_t dim) {
   w.order = take(n * 4);
   w.starts = take(((w.share << w.log_shares) + 1) * 4);
   // In one launch, split: 8192 tokens 10.5 and 11.3 us (256 rows), 11.4 and 13.1 (131072 rows); 12288 tokens 16.4 and 12.1, 16.0 and 13.9; 65536
-  // tokens 67 and 29, 66 and 19. With more shares or tiles than LDS holds: one launch.
+  // tokens 67 and 29, 66 and 19. With more shares (more than 2^18 rows) or tiles (more than 2^20 tokens) than LDS holds: one launch, and every
+  // share's workgroup reads all tokens.
   w.tiles = static_cast<int>((n + kTile - 1) / kTile);
   w.split = n > kOneLaunch && n <= int64_t(kTile) * kMostTiles && w.log_shares <= 9;
   if (w.split) {
