@@ -194,3 +194,49 @@ def test_a_lookup_writes_its_rows_and_nothing_else(vocab, dim, n, dtype, lead):
     _lib.check(_lib.lib().tdm_k5_embedding(w.data_ptr(), tokens.data_ptr(), 4, out.data_ptr(), n, vocab, dim, ops.CODES[dtype], 1.0, torch.cuda.current_stream().cuda_stream))
     assert torch.equal(out.view(n, dim), w[tokens])
     assert (around[:64 + lead] == 7).all() and (around[64 + lead + n * dim:] == 7).all()
+
+
+def test_a_compiled_program_calls_the_operators():
+    """torch.compile leaves its graph for every launch: same losses and gradients, twice, and with other inputs."""
+    from tandem_amd import ops
+
+    gen = torch.Generator().manual_seed(11)
+    table, proj, qw, kw = (torch.randn(*s, generator=gen).mul_(0.1).to(DEV).requires_grad_() for s in ((50, 32), (64, 32), (16,), (16,)))
+    freq, pos = ops.rope_frequencies(16), torch.arange(6, device=DEV)
+
+    def program(tokens, columns, teacher):
+        x = ops.embedding(tokens, table, scale=2.0)
+        q, k, v = ops.qkv_norm_rope(x @ proj.t(), 2, 1, qw, kw, pos, freq)
+        logits = torch.cat((q.flatten(2), k.flatten(2), v.flatten(2)), -1) * 3
+        return ops.distill_loss(logits, columns, teacher, temperature=2.0) / 2
+
+    compiled = torch.compile(program, backend="eager")
+    for seed in (1, 2, 3):
+        gen.manual_seed(seed)
+        inputs = torch.randint(0, 50, (2, 6), generator=gen).to(DEV), torch.randint(0, 64, (2, 6, 3), generator=gen).to(DEV), torch.randn(2, 6, 3, generator=gen).to(DEV)
+        leaves = (table, proj, qw, kw)
+        want_loss = program(*inputs)
+        want = torch.autograd.grad(want_loss, leaves)
+        loss = compiled(*inputs)
+        assert torch.equal(loss, want_loss) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, leaves), want))
+
+
+def test_what_is_refused_on_the_gpu_too():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from tandem_amd import ops
+
+    w, tokens = torch.randn(9, 4, device=DEV), torch.tensor([1, 2], device=DEV)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        ops.embedding(tokens, forward_ad.make_dual(w, torch.ones_like(w)))
+    for record in (lambda: torch.jit.trace(lambda w: ops.embedding(tokens, w), (w,)), lambda: make_fx(lambda w: ops.embedding(tokens, w))(w)):
+        with pytest.raises(NotImplementedError, match="recorded"):
+            record()
+    with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+        torch.func.jvp(lambda w: ops.embedding(tokens, w), (w,), (torch.ones_like(w),))
+    leaf = w.clone().requires_grad_()
+    out = ops.embedding(tokens, leaf)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+    assert torch.equal(ops.embedding(tokens, w), w[tokens])
